@@ -4,7 +4,7 @@ set -e
 cd "$(dirname "$0")"
 OUT=../lib
 mkdir -p $OUT _obj
-FLAGS="--offload-arch=gfx950 -O3 -fPIC -std=c++17 -fvisibility=hidden -Wall -Wno-unused-function"
+FLAGS="--offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -fPIC -std=c++17 -fvisibility=hidden -Wall -Wno-unused-function"
 pids=()
 for f in *.hip; do
   o=_obj/${f%.hip}.o
