@@ -124,5 +124,38 @@ def ptr(t):
     return t.data_ptr()
 
 
+def rows_ptr(t, what, dtypes, cols=None):
+    """(device pointer, row stride) of a 2-D GPU tensor on the current device whose rows are contiguous and do not overlap."""
+    if not isinstance(t, torch.Tensor) or t.dim() != 2 or t.dtype not in dtypes or (cols is not None and t.shape[1] != cols):
+        got = f"{tuple(t.shape)} {t.dtype}" if isinstance(t, torch.Tensor) else repr(t)
+        raise SwatHipError(f"{what}: a 2-D tensor{'' if cols is None else f' of {cols} columns'} in "
+                           f"{' or '.join(str(d)[6:] for d in dtypes)} is wanted, got {got}")
+    on_device(t, what)
+    rows, n = t.shape
+    ld = t.stride(0) if rows > 1 else n
+    if (n > 1 and t.stride(1) != 1) or ld < n:
+        raise SwatHipError(f"{what}: rows have to be contiguous and apart, got strides {t.stride()}")
+    return t.data_ptr(), ld
+
+
+def vec_ptr(t, what, n):
+    """Device pointer of a contiguous fp32 tensor of shape n (or None)."""
+    if t is None:
+        return None
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or tuple(t.shape) != n or not t.is_contiguous():
+        got = f"{tuple(t.shape)} {t.dtype}" if isinstance(t, torch.Tensor) else repr(t)
+        raise SwatHipError(f"{what}: a contiguous float32 tensor of shape {n} is wanted, got {got}")
+    on_device(t, what)
+    return t.data_ptr()
+
+
+def on_device(t, what):
+    """Kernels launch on the current device's current stream: a tensor elsewhere is refused instead of read from there."""
+    if not t.is_cuda:
+        raise SwatHipError(f"{what}: swat_amd ops need GPU tensors (no CPU fallback)")
+    if t.device.index != torch.cuda.current_device():
+        raise SwatHipError(f"{what}: tensor on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
 def stream():
     return torch.cuda.current_stream().cuda_stream

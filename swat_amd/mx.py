@@ -1,0 +1,135 @@
+"""Microscaled matrices: blocks of 32 columns of a row share a power of two, elements are e4m3 (8 bits) or e2m1 (4 bits).
+
+8 bits are the checkpoint form of activations — a linear layer's input, an MLP's pre-activation — that the backward pass reads as
+they are (linear_wgrad, act_bwd); 4 bits halve that again for weights of frozen towers and large collections of rows; matmul
+multiplies any two of them without unpacking.  Thin wrappers over the C ABI (include/swat_hip.h) on torch's current stream; no
+PyTorch fallback.
+"""
+from collections import namedtuple
+
+import torch
+
+from . import _lib
+from ._lib import ptr as _p
+from .ops import ACT
+
+_BF, _F32 = torch.bfloat16, torch.float32
+
+
+class MX(namedtuple("MX", "codes scale cols bits")):
+    """A packed [rows, cols] matrix: codes uint8 [rows, ceil(cols / 32) * 32 * bits / 8] (4 bits: the even column in the low half, zeros
+    behind the last column), scale uint8 [rows, ceil(cols / 32)] (exponent + 127; 255: the block is NaN)."""
+    __slots__ = ()
+
+    @property
+    def rows(self):
+        return self.codes.shape[0]
+
+    @property
+    def shape(self):
+        return (self.codes.shape[0], self.cols)
+
+
+def _empty(rows, cols, bits, dev):
+    blocks = (cols + 31) // 32
+    return MX(torch.empty((rows, blocks * 4 * bits), dtype=torch.uint8, device=dev), torch.empty((rows, blocks), dtype=torch.uint8, device=dev),
+              cols, bits)
+
+
+def _check(m, what, bits=(4, 8)):
+    if not isinstance(m, MX) or m.bits not in bits or m.cols < 1:
+        raise _lib.SwatHipError(f"{what}: an MX matrix of {' or '.join(map(str, bits))} bits is wanted, got {m!r:.80}")
+    rows, blocks = m.codes.shape[0], (m.cols + 31) // 32
+    if (m.codes.dtype != torch.uint8 or m.scale.dtype != torch.uint8 or m.codes.shape != (rows, blocks * 4 * m.bits)
+            or m.scale.shape != (rows, blocks)):
+        raise _lib.SwatHipError(f"{what}: codes {tuple(m.codes.shape)} {m.codes.dtype} and scale {tuple(m.scale.shape)} {m.scale.dtype} are not "
+                                f"those of {m.cols} columns in {m.bits} bits")
+    _lib.on_device(m.codes, what)
+    _lib.on_device(m.scale, what)
+    return _p(m.codes), _p(m.scale)
+
+
+def _act(act, what):
+    if ACT.get(act, 0) == 0:
+        raise _lib.SwatHipError(f"{what}: activation {act!r} ('gelu' or 'quick_gelu')")
+    return ACT[act]
+
+
+def quantize(x, bits=8):
+    """x [rows, cols] bf16 or fp32 (rows may be strided) -> MX."""
+    px, ld = _lib.rows_ptr(x, "mx.quantize", (_BF, _F32))
+    if bits not in (4, 8) or x.shape[1] < 1:
+        raise _lib.SwatHipError(f"mx.quantize: {bits} bits (4 or 8) of {x.shape[1]} columns (1 at least)")
+    m = _empty(x.shape[0], x.shape[1], bits, x.device)
+    _lib.check(_lib.lib().swat_mx_quantize(px, ld, int(x.dtype == _BF), bits, _p(m.codes), _p(m.scale), x.shape[0], x.shape[1], _lib.stream()),
+               "swat_mx_quantize")
+    return m
+
+
+def dequantize(m, dtype=_BF):
+    """The values an MX matrix stands for, [rows, cols] in bf16 or fp32 (exact in both)."""
+    codes, scale = _check(m, "mx.dequantize")
+    if dtype not in (_BF, _F32):
+        raise _lib.SwatHipError(f"mx.dequantize: {dtype} (bfloat16 or float32)")
+    out = torch.empty(m.shape, dtype=dtype, device=m.codes.device)
+    _lib.check(_lib.lib().swat_mx_dequantize(codes, scale, m.bits, _p(out), int(dtype == _BF), m.rows, m.cols, _lib.stream()),
+               "swat_mx_dequantize")
+    return out
+
+
+def act_fwd(f, act="gelu"):
+    """f bf16 [rows, n] -> (act(f) bf16, the 8-bit checkpoint of f), f read once."""
+    pf, ld = _lib.rows_ptr(f, "mx.act_fwd", (_BF,))
+    a = _act(act, "mx.act_fwd")
+    if f.shape[1] < 1:
+        raise _lib.SwatHipError("mx.act_fwd: no columns")
+    m = _empty(f.shape[0], f.shape[1], 8, f.device)
+    g = torch.empty(f.shape, dtype=_BF, device=f.device)
+    _lib.check(_lib.lib().swat_mx_act_fwd(pf, ld, a, _p(g), _p(m.codes), _p(m.scale), f.shape[0], f.shape[1], _lib.stream()), "swat_mx_act_fwd")
+    return g, m
+
+
+def act_bwd(dg, m, act="gelu", want_act=True):
+    """dg bf16 [rows, n] and the checkpoint of f -> (df = dg act'(f8) bf16, act(f8) bf16 or None)."""
+    codes, scale = _check(m, "mx.act_bwd", (8,))
+    pg, ld = _lib.rows_ptr(dg, "mx.act_bwd: dg", (_BF,), m.cols)
+    a = _act(act, "mx.act_bwd")
+    if dg.shape[0] != m.rows:
+        raise _lib.SwatHipError(f"mx.act_bwd: {dg.shape[0]} rows of dg, {m.rows} of the checkpoint")
+    df = torch.empty(m.shape, dtype=_BF, device=dg.device)
+    g = torch.empty(m.shape, dtype=_BF, device=dg.device) if want_act else None
+    _lib.check(_lib.lib().swat_mx_act_bwd(pg, ld, codes, scale, a, _p(df), _p(g), m.rows, m.cols, _lib.stream()), "swat_mx_act_bwd")
+    return df, g
+
+
+def linear_wgrad(dy, m, want_bias=False, out=None):
+    """Weight gradient from the 8-bit checkpoint of a linear layer's input: dy bf16 [rows, n] -> dW fp32 [n, cols] (, column sums of dy)."""
+    codes, scale = _check(m, "mx.linear_wgrad", (8,))
+    py, ld = _lib.rows_ptr(dy, "mx.linear_wgrad: dy", (_BF,))
+    rows, n = dy.shape
+    if rows != m.rows:
+        raise _lib.SwatHipError(f"mx.linear_wgrad: {rows} rows of dy, {m.rows} of the checkpoint")
+    if out is None:
+        out = torch.empty((n, m.cols), dtype=_F32, device=dy.device)
+    pw = _lib.vec_ptr(out, "mx.linear_wgrad: out", (n, m.cols))
+    db = torch.empty(n, dtype=_F32, device=dy.device) if want_bias else None
+    h = _lib.lib()
+    nbytes = h.swat_mx_linear_wgrad_workspace_bytes(rows, n, m.cols)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dy.device) if nbytes > 0 else None
+    _lib.check(h.swat_mx_linear_wgrad(py, ld, codes, scale, pw, _p(db), rows, n, m.cols, _p(ws), nbytes, _lib.stream()), "swat_mx_linear_wgrad")
+    return (out, db) if want_bias else out
+
+
+def matmul(a, b, bias=None, out_dtype=_BF):
+    """a [M, K] @ b [N, K].T (+ bias fp32 [N]) -> [M, N]; 4 or 8 bits each, nothing is unpacked.  bf16, or fp32 where both have 4 bits
+    (with an 8-bit operand the matrix instruction keeps 13 binary places below the largest of eight neighbouring products)."""
+    ca, sa = _check(a, "mx.matmul: a")
+    cb, sb = _check(b, "mx.matmul: b")
+    if a.cols != b.cols or not (out_dtype == _BF or (out_dtype == _F32 and a.bits == b.bits == 4)):
+        raise _lib.SwatHipError(f"mx.matmul: {a.shape} in {a.bits} bits by {b.shape} in {b.bits} bits (the same columns) into {out_dtype} "
+                                "(bfloat16; float32 where both have 4 bits)")
+    pb = _lib.vec_ptr(bias, "mx.matmul: bias", (b.rows,))
+    c = torch.empty((a.rows, b.rows), dtype=out_dtype, device=a.codes.device)
+    _lib.check(_lib.lib().swat_mx_matmul(ca, sa, a.bits, cb, sb, b.bits, pb, _p(c), int(out_dtype == _BF), a.rows, b.rows, a.cols, _lib.stream()),
+               "swat_mx_matmul")
+    return c
