@@ -4,99 +4,229 @@
 //
 // dY bfloat16, X8 e4m3 with a power-of-two scale to 32 columns.  An e4m3 number times such a scale is a bfloat16 number, so the
 // checkpoint is unpacked on its way into LDS without a rounding and v_mfma_f32_16x16x32_bf16 sees what was stored.  The reduction
-// runs over rows: both tiles lie [64 rows][128 columns] in LDS and are read with the transposing LDS load.
+// runs over rows: both tiles lie [64 rows][columns] in LDS and are read with the transposing LDS load.
+//
+// Bound by the matrix cores where it is large: 16448 rows, 4096 x 1024 takes 150 us (920 TFLOP/s; the large bf16 library product 1 425, the
+// same gradient from a bf16 input 149-179 with the GEMM kernels of gemm_*.hip), matrix pipes busy 44 % of the time by counter.  A wave's
+// 64 x 64 and 8 waves to a CU leave one other wave to a SIMD to cover LDS reads, LDS writes and the unpacking; wider wave tiles spilled.
+// The long side of the tile goes to X because its codes are half as many bytes: 32 KB instead of 40 from memory for the same products.
+#include <math.h>
 #include "gemm_device.hpp"
 #include "mx_device.hpp"
 #include "../../include/swat_hip.h"
 
 namespace swat {
 
+typedef unsigned mx_u4 __attribute__((ext_vector_type(4)));
+
 struct MxWgradArgs {
     const unsigned short* dY;
     const unsigned char *X, *S;
-    float *dW, *db;
+    float *dW, *db;     // or the partial planes of a split reduction
     int64_t rows, ld;   // rows; row stride of dY
     int n, k, blocks;
-    int tiles_n, tiles_k;
-    int vec;            // dY rows on 16 bytes, n % 8 == 0
+    int tiles_n, tiles_k, splits, tiles_per_split;   // 64-row tiles to a split
 };
 
-__global__ __launch_bounds__(256) void mx_wgrad_kernel(MxWgradArgs p) {
-    __shared__ __attribute__((aligned(1024))) unsigned char ty[64 * 256], tx[64 * 256];
+// A workgroup computes BN x BK of dW over its share of the rows; waves of WN x WK.  64 rows at a time: both operands go through
+// registers into one of two LDS buffers ([64 rows][columns], 16-byte chunks permuted so that neither the writes nor the transposing
+// reads meet in a bank) while the matrix cores work on the other; the global loads run a whole tile ahead.
+template <int BN, int BK, int WN, int WK>
+__global__ __launch_bounds__((BN / WN) * (BK / WK) * 64, 2) void mx_wgrad_kernel(MxWgradArgs p) {
+    constexpr int NT = (BN / WN) * (BK / WK) * 64, FN = WN / 16, FK = WK / 16;
+    constexpr int YB = 64 * BN * 2, XB = 64 * BK * 2;
+    constexpr int YC = 64 * BN / 8 / NT, XC = 64 * BK / 16 / NT;   // chunks to a thread: 8 columns of dY, 16 of X
+    static_assert(YC * NT * 8 == 64 * BN && XC * NT * 16 == 64 * BK, "whole chunks");
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * (YB + XB)];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int r16 = lane & 15, g = lane >> 4, wr = wave >> 1, wc = wave & 1;
-    const int n0 = (blockIdx.x % p.tiles_n) * 128, k0 = (blockIdx.x / p.tiles_n) * 128;
-    f32x4_t acc[4][4], accs[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        accs[i] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+    const int r16 = lane & 15, g = lane >> 4, wr = wave / (BK / WK), wc = wave % (BK / WK);
+    // units of one XCD (workgroups b, b + 8, ..) are neighbours: the same rows, 4 k tiles wide, so that its L2 sees few panels of dY and X
+    int id;
+    {
+        const int total = gridDim.x, xcd = blockIdx.x & 7, q = total >> 3, r = total & 7;
+        id = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (blockIdx.x >> 3);
     }
-    const bool sums = p.db && k0 == 0 && wc == 0;
-    bf16x8_t ones;
+    const int tiles = p.tiles_n * p.tiles_k, split = id / tiles, in = id - split * tiles;
+    const int band = in / (4 * p.tiles_n), wide = p.tiles_k - 4 * band < 4 ? p.tiles_k - 4 * band : 4;
+    const int tk = 4 * band + (in - 4 * band * p.tiles_n) % wide, tn = (in - 4 * band * p.tiles_n) / wide;
+    const int n0 = tn * BN, k0 = tk * BK;
+    const int64_t t0 = (int64_t)split * p.tiles_per_split, all = (p.rows + 63) / 64;
+    const int nt = (int)(t0 + p.tiles_per_split < all ? p.tiles_per_split : all > t0 ? all - t0 : 0);
+
+    // Global loads go through buffer descriptors that end with the matrix: rows past the last one read as zeros, columns past the edge get
+    // an offset past the end.  dY may sit on any 2 bytes; the range check is by whole dwords, so with an odd n the matrix's very last
+    // element reads as zero too: its products are added at the end.  A thread's offsets inside a tile are constant, the tile's base advances in scalar registers.
+    struct Stage {
+        mx_u4 y[YC], x[XC];
+        unsigned char s[XC];
+    };
+    Stage st0, st1;
+    float cs[8];   // this thread's 8 columns of dY, summed over its rows (at % (BN / 8) is the same for all its chunks)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) ones[e] = (__bf16)1.0f;
-    for (int64_t m0 = 0; m0 < p.rows; m0 += 64) {
-        __syncthreads();
+    for (int e = 0; e < 8; ++e) cs[e] = 0.f;
+    const bool sums = p.db && tk == 0;
+    const int xld = 32 * p.blocks;
+    constexpr unsigned OUT = 0x80000000u;
+    // (a thread's chunks are YR (XR) rows apart, multiples of 16: the permutation of 16-byte chunks in LDS is the same for all of them)
+    constexpr int YR = NT / (BN / 8), XR = NT / (BK / 16), YW = BN >= 128 ? 256 : 2 * BN, XW = BK >= 128 ? 256 : 2 * BK;
+    static_assert(YR % 16 == 0 && XR % 16 == 0, "rows between a thread's chunks");
+    const int yrow = tid / (BN / 8), ycol = n0 + 8 * (tid % (BN / 8)), xrow = tid / (BK / 16), xcol = k0 + 16 * (tid % (BK / 16));
+    const unsigned oy = ycol < p.n ? 2u * (unsigned)(yrow * (int)p.ld + ycol) : OUT, ox = xcol < xld ? (unsigned)(xrow * xld + xcol) : OUT;
+    const unsigned os = xcol < xld ? (unsigned)(xrow * p.blocks + (xcol >> 5)) : OUT;
+    unsigned char *const wy = smem + stp_off<BN>(yrow, ycol - n0), *const wx = smem + 2 * YB + stp_off<BK>(xrow, xcol - k0);
+    auto load = [&](Stage& st, int t) {
+        const int64_t m0 = (t0 + t) * 64 < p.rows ? (t0 + t) * 64 : p.rows, left = p.rows - m0;
+        const int rows = left < 64 ? (int)left : 64;   // (a tile with rows behind it: one element more, its last dword may reach into the next)
+        const __amdgpu_buffer_rsrc_t by = __builtin_amdgcn_make_buffer_rsrc((void*)(p.dY + m0 * p.ld), 0,
+                                                                             left > 64 ? 128 * (int)p.ld + 2 : rows ? 2 * ((rows - 1) * (int)p.ld + p.n) : 0, 0x20000);
+        const __amdgpu_buffer_rsrc_t bx = __builtin_amdgcn_make_buffer_rsrc((void*)(p.X + m0 * xld), 0, rows * xld, 0x20000);
+        const __amdgpu_buffer_rsrc_t bs = __builtin_amdgcn_make_buffer_rsrc((void*)(p.S + m0 * p.blocks), 0, rows * p.blocks, 0x20000);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int at = i * 256 + tid, row = at >> 4, c = at & 15;   // 16 chunks of 8 columns to a row
-            const int64_t m = m0 + row;
-            {
-                const int col = n0 + 8 * c;
-                uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                if (m < p.rows && col < p.n) {
-                    const unsigned short* src = p.dY + m * p.ld + col;
-                    if (p.vec) v = *reinterpret_cast<const uint4*>(src);
-                    else {
-                        unsigned w[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            if (col + e < p.n) w[e >> 1] |= (unsigned)src[e] << (16 * (e & 1));
-                        v = make_uint4(w[0], w[1], w[2], w[3]);
-                    }
-                }
-                *reinterpret_cast<uint4*>(ty + st_off<128>(row, c)) = v;
-            }
-            {
-                const int col = k0 + 8 * c;
-                uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                if (m < p.rows && col < 32 * p.blocks) {
-                    const uint2 q = *reinterpret_cast<const uint2*>(p.X + m * (32 * (int64_t)p.blocks) + col);
-                    const float s = mx_scale(p.S[m * p.blocks + (col >> 5)]);
-                    float f[8];
-                    mx_from_e4m3x4(q.x, s, f);
-                    mx_from_e4m3x4(q.y, s, f + 4);
-                    v = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
-                }
-                *reinterpret_cast<uint4*>(tx + st_off<128>(row, c)) = v;
-            }
+        for (int i = 0; i < YC; ++i) {
+            st.y[i] = __builtin_amdgcn_raw_buffer_load_b128(by, oy + 2u * (unsigned)(i * YR * (int)p.ld), 0, 0);
         }
-        __syncthreads();
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-            bf16x8_t fx[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) fx[j] = read_frag<false, 128>(tx, 64 * wc + 16 * j, ks, lane);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const bf16x8_t fy = read_frag<false, 128>(ty, 64 * wr + 16 * i, ks, lane);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fx[j], fy, acc[i][j], 0, 0, 0);
-                if (sums) accs[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, fy, accs[i], 0, 0, 0);
-            }
+        for (int i = 0; i < XC; ++i) {
+            st.x[i] = __builtin_amdgcn_raw_buffer_load_b128(bx, ox + (unsigned)(i * XR * xld), 0, 0);
+            st.s[i] = __builtin_amdgcn_raw_buffer_load_b8(bs, os + (unsigned)(i * XR * p.blocks), 0, 0);
         }
+    };
+    auto put = [&](Stage& st, int buf, bool mine) {
+#pragma unroll
+        for (int i = 0; i < YC; ++i) *reinterpret_cast<mx_u4*>(wy + buf * YB + i * YR * YW) = st.y[i];
+        if (mine) {
+#pragma unroll
+            for (int i = 0; i < YC; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    cs[2 * e] += __uint_as_float(st.y[i][e] << 16);
+                    cs[2 * e + 1] += __uint_as_float(st.y[i][e] & 0xffff0000u);
+                }
+        }
+#pragma unroll
+        for (int i = 0; i < XC; ++i) {
+            const float s = mx_scale(st.s[i]);
+            unsigned w[8];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {   // exact: an e4m3 number times a power of two of at least 2^-110
+                w[2 * e] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(st.x[i][e], s, false));
+                w[2 * e + 1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(st.x[i][e], s, true));
+            }
+            // (a quarter wave covers 256 bytes in two writes: lanes 4 .. 7 of each eight write their second half first, so that eight
+            // lanes meet all banks once)
+            const bool late = tid & 4;
+            *reinterpret_cast<mx_u4*>(wx + buf * XB + i * XR * XW + (late ? 16 : 0)) =
+                late ? (mx_u4){w[4], w[5], w[6], w[7]} : (mx_u4){w[0], w[1], w[2], w[3]};
+            *reinterpret_cast<mx_u4*>(wx + buf * XB + i * XR * XW + (late ? 0 : 16)) =
+                late ? (mx_u4){w[0], w[1], w[2], w[3]} : (mx_u4){w[4], w[5], w[6], w[7]};
+        }
+    };
+    auto bar = [&]() {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    // fragment of 8 rows of one column: lane (r16, g) of the 32-row half ks gets rows 32 ks + 8 g + 0 .. 7 of column base + r16
+    auto frag = [&](const unsigned char* lo, int row_bytes) {
+        const s16x4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(lo));
+        const s16x4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(lo + 4 * row_bytes));
+        const s16x8_t v = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+        return __builtin_bit_cast(bf16x8_t, v);
+    };
+
+    f32x4_t acc[FN][FK];
+#pragma unroll
+    for (int i = 0; i < FN; ++i)
+#pragma unroll
+        for (int j = 0; j < FK; ++j) acc[i][j] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+
+    struct Frags {
+        bf16x8_t x[FK], y[FN];
+    };
+    Frags f0, f1;   // of the two 32-row halves of a tile
+    // (the permutation depends on the low four bits of the row with bit 2 left out: rows + 4 and + 32 are at constant distances)
+    const unsigned char *rx[FK], *ry[FN];
+#pragma unroll
+    for (int j = 0; j < FK; ++j) rx[j] = smem + 2 * YB + 8 * (r16 & 3) + stp_off<BK>(8 * g + (r16 >> 2), WK * wc + 16 * j);
+#pragma unroll
+    for (int i = 0; i < FN; ++i) ry[i] = smem + 8 * (r16 & 3) + stp_off<BN>(8 * g + (r16 >> 2), WN * wr + 16 * i);
+    auto read = [&](Frags& f, int buf, int ks) {
+#pragma unroll
+        for (int j = 0; j < FK; ++j) f.x[j] = frag(rx[j] + buf * XB + ks * 32 * XW, XW);
+#pragma unroll
+        for (int i = 0; i < FN; ++i) f.y[i] = frag(ry[i] + buf * YB + ks * 32 * YW, YW);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto multiply = [&](Frags& f) {
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int i = 0; i < FN; ++i)
+#pragma unroll
+            for (int j = 0; j < FK; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.x[j], f.y[i], acc[i][j], 0, 0, 0);
+        __builtin_amdgcn_s_setprio(0);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // One barrier to a tile: a half's fragments are read while the matrix cores work on the half before; tile t + 1 goes into the other
+    // buffer in between (whose last reads were waited for at the barrier before), t + 2 and t + 3 are on their way from memory.
+    // Nothing in the loop is conditional (tiles past this split's last one are loaded, and past the matrix read as zeros, but not
+    // multiplied): the waits for the loads stay exact.
+    auto step = [&](Stage& st, int buf, int t) {
+        read(f1, buf, 1);
+        multiply(f0);
+        put(st, buf ^ 1, sums && t + 1 < nt);
+        load(st, t + 3);
+        bar();
+        read(f0, buf ^ 1, 0);
+        multiply(f1);
+    };
+    load(st0, 0);
+    load(st1, 1);
+    put(st0, 0, sums && nt > 0);
+    load(st0, 2);
+    bar();
+    read(f0, 0, 0);
+    int t = 0;
+    for (; t + 1 < nt; t += 2) {
+        step(st1, 0, t);
+        step(st0, 1, t + 1);
     }
+    if (t < nt) {
+        read(f1, 0, 1);
+        multiply(f0);
+        multiply(f1);
+    }
+    bar();
+    const bool odd_end = (p.n & 1) && nt > 0 && t0 + nt == all;   // (see the loads)
+    if (sums) {   // the threads that share 8 columns meet in LDS (tiles are done with it), rows of threads added in order
+        float* cp = reinterpret_cast<float*>(smem);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int n = n0 + 64 * wr + 16 * i + r16;
+        for (int e = 0; e < 8; ++e) cp[(tid / (BN / 8)) * BN + 8 * (tid % (BN / 8)) + e] = cs[e];
+        bar();
+        for (int c = tid; c < BN; c += NT)
+            if (n0 + c < p.n) {
+                float t = 0.f;
+#pragma unroll
+                for (int r = 0; r < NT / (BN / 8); ++r) t += cp[r * BN + c];
+                if (odd_end && n0 + c == p.n - 1) t += bf2f(p.dY[(p.rows - 1) * p.ld + n0 + c]);
+                p.db[(int64_t)split * p.n + n0 + c] = t;
+            }
+    }
+    float* dW = p.dW + (int64_t)split * p.n * p.k;
+#pragma unroll
+    for (int i = 0; i < FN; ++i) {
+        const int n = n0 + WN * wr + 16 * i + r16;
         if (n >= p.n) continue;
-        if (sums && g == 0) p.db[n] = accs[i][0];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int k = k0 + 64 * wc + 16 * j + 4 * g;
-            float* out = p.dW + (int64_t)n * p.k + k;
+        for (int j = 0; j < FK; ++j) {
+            const int k = k0 + WK * wc + 16 * j + 4 * g;
+            if (odd_end && n == p.n - 1 && k < xld) {
+                const float y = bf2f(p.dY[(p.rows - 1) * p.ld + n]);
+                float x[4];
+                mx_from_e4m3x4(*reinterpret_cast<const unsigned*>(p.X + (p.rows - 1) * xld + k), mx_scale(p.S[(p.rows - 1) * p.blocks + (k >> 5)]), x);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(y, x[e], acc[i][j][e]);
+            }
+            float* out = dW + (int64_t)n * p.k + k;
             if (p.k % 4 == 0) {
                 if (k < p.k) *reinterpret_cast<float4*>(out) = make_float4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]);
             } else {
@@ -108,26 +238,106 @@ __global__ __launch_bounds__(256) void mx_wgrad_kernel(MxWgradArgs p) {
     }
 }
 
+// the planes of a split reduction, added in their order: dW behind which db follows in planes of its own
+__global__ __launch_bounds__(256) void mx_wgrad_join_kernel(const float* pw, const float* pb, float* dW, float* db, int64_t nk, int n, int splits, int vec) {
+    const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (at < nk) {
+        if (vec) {
+            float4 s = *reinterpret_cast<const float4*>(pw + at);
+            for (int i = 1; i < splits; ++i) {
+                const float4 t = *reinterpret_cast<const float4*>(pw + i * nk + at);
+                s.x += t.x; s.y += t.y; s.z += t.z; s.w += t.w;
+            }
+            *reinterpret_cast<float4*>(dW + at) = s;
+        } else {
+            for (int e = 0; e < 4 && at + e < nk; ++e) {
+                float s = pw[at + e];
+                for (int i = 1; i < splits; ++i) s += pw[i * nk + at + e];
+                dW[at + e] = s;
+            }
+        }
+    }
+    if (db && at < n)
+        for (int e = 0; e < 4 && at + e < n; ++e) {
+            float s = pb[at + e];
+            for (int i = 1; i < splits; ++i) s += pb[(int64_t)i * n + at + e];
+            db[at + e] = s;
+        }
+}
+
+struct MxWgradPlan {
+    int big, tiles_n, tiles_k, splits, per;
+};
+// 128 x 256 tiles (8 waves, one workgroup to a CU) or 64 x 64 (4 waves, up to four), and into how many parts the rows are split, by the
+// sum of what was measured (us): a 64-row tile takes 1.02 in the first form; in the second 0.43 alone on its CU and 0.27 for each of
+// several; 6.5 / 3 to start and to store; a join 2.5 and its planes' bytes at 4.5 TB/s.  At 16448 rows, 4096 x 1024: 150 in the first
+// form with 2 parts (259 with 1, 157 with 4), 240 in the second; at 1600 rows, 768 x 768: 13.7 in the second (1 part), 21.4 in the first.
+static MxWgradPlan mx_wgrad_plan(int64_t rows, int n, int k) {
+    const int64_t all = (rows + 63) / 64;
+    MxWgradPlan best = {};
+    double cost = -1;
+    for (int big = 0; big < 2; ++big) {
+        const int bn = big ? 128 : 64, bk = big ? 256 : 64;
+        MxWgradPlan p = {big, (n + bn - 1) / bn, (k + bk - 1) / bk, 1, 1};
+        for (int s = 1; s <= 16 && (s == 1 || s <= all); ++s) {
+            p.per = all > 0 ? (int)((all + s - 1) / s) : 1;
+            p.splits = all > 0 ? (int)((all + p.per - 1) / p.per) : 1;
+            if (p.splits != s) continue;
+            const double units = (double)p.tiles_n * p.tiles_k * s, rounds = ceil(units / (big ? 256 : 1024));
+            const double at_once = units > 1024 ? 4 : ceil(units / 256);
+            const double tile = big ? 1.02 : at_once < 2 ? 0.43 : 0.27 * at_once;
+            const double c = (big ? 6.5 : 3.0) + rounds * p.per * tile + (s > 1 ? 2.5 + (s + 1.0) * n * k * 4 / 4.5e6 : 0.0);
+            if (cost < 0 || c < cost) {
+                cost = c;
+                best = p;
+            }
+        }
+    }
+    return best;
+}
+
 }  // namespace swat
 
 using namespace swat;
 
-SWAT_API int64_t swat_mx_linear_wgrad_workspace_bytes(int64_t rows, int n_out, int n_in) { return 0; }
+SWAT_API int64_t swat_mx_linear_wgrad_workspace_bytes(int64_t rows, int n_out, int n_in) {
+    if (rows < 0 || rows >= (1ll << 36) || n_out < 0 || n_in < 0 || n_out > (1 << 23) || n_in > (1 << 24)) {
+        set_error("swat_mx_linear_wgrad_workspace_bytes: %lld rows, %d x %d", (long long)rows, n_out, n_in);
+        return -1;
+    }
+    const MxWgradPlan p = mx_wgrad_plan(rows, n_out, n_in);
+    return p.splits > 1 ? 4 * (int64_t)p.splits * n_out * ((int64_t)n_in + 1) : 0;
+}
 
 SWAT_API int swat_mx_linear_wgrad(const void* dY_bf16, int64_t dy_stride, const void* x_codes, const void* x_scales, float* dW, float* dbias,
                                   int64_t rows, int n_out, int n_in, void* workspace, int64_t workspace_bytes, swat_stream_t stream) {
-    SWAT_REQUIRE(rows >= 0 && n_out >= 0 && n_in >= 0 && n_out <= (1 << 24) && n_in <= (1 << 24), "swat_mx_linear_wgrad: %lld rows, %d x %d", (long long)rows, n_out, n_in);
+    SWAT_REQUIRE(rows >= 0 && rows < (1ll << 36) && n_out >= 0 && n_in >= 0 && n_out <= (1 << 23) && n_in <= (1 << 24), "swat_mx_linear_wgrad: %lld rows, %d x %d", (long long)rows, n_out, n_in);
     if (n_out == 0 || n_in == 0) return 0;
     SWAT_REQUIRE(dW && (rows == 0 || (dY_bf16 && x_codes && x_scales)), "swat_mx_linear_wgrad: dY, the checkpoint and dW are needed");
     SWAT_REQUIRE(rows == 0 || dy_stride >= n_out, "swat_mx_linear_wgrad: row stride %lld under %d columns", (long long)dy_stride, n_out);
+    SWAT_REQUIRE(rows == 0 || dy_stride <= (1 << 23), "swat_mx_linear_wgrad: row stride %lld past 2^23", (long long)dy_stride);
     SWAT_REQUIRE(!(((uintptr_t)x_codes | (uintptr_t)dW) & 15), "swat_mx_linear_wgrad: codes and dW sit on 16 bytes");
+    const MxWgradPlan pl = mx_wgrad_plan(rows, n_out, n_in);
+    const int64_t grid = (int64_t)pl.tiles_n * pl.tiles_k * pl.splits, nk = (int64_t)n_out * n_in;
+    SWAT_REQUIRE(grid < (1ll << 31) && nk < (1ll << 40), "swat_mx_linear_wgrad: %d x %d is past one launch", n_out, n_in);
+    const int64_t want = swat_mx_linear_wgrad_workspace_bytes(rows, n_out, n_in);
+    SWAT_REQUIRE(want == 0 || (workspace && workspace_bytes >= want && ((uintptr_t)workspace & 15) == 0),
+                 "swat_mx_linear_wgrad: workspace of %lld bytes, %lld on 16 bytes are needed", (long long)workspace_bytes, (long long)want);
+    const hipStream_t s = (hipStream_t)stream;
+    float *pw = dW, *pb = dbias;
+    if (pl.splits > 1) {
+        pw = (float*)workspace;
+        pb = dbias ? pw + pl.splits * nk : nullptr;
+    }
     MxWgradArgs p = {};
-    p.dY = (const unsigned short*)dY_bf16; p.X = (const unsigned char*)x_codes; p.S = (const unsigned char*)x_scales; p.dW = dW; p.db = dbias;
+    p.dY = (const unsigned short*)dY_bf16; p.X = (const unsigned char*)x_codes; p.S = (const unsigned char*)x_scales; p.dW = pw; p.db = pb;
     p.rows = rows; p.ld = dy_stride; p.n = n_out; p.k = n_in; p.blocks = (n_in + 31) / 32;
-    p.vec = n_out % 8 == 0 && dy_stride % 8 == 0 && ((uintptr_t)dY_bf16 & 15) == 0;
-    p.tiles_n = (n_out + 127) / 128; p.tiles_k = (n_in + 127) / 128;
-    const int64_t grid = (int64_t)p.tiles_n * p.tiles_k;
-    SWAT_REQUIRE(grid < (1ll << 31), "swat_mx_linear_wgrad: %d x %d is past one launch", n_out, n_in);
-    mx_wgrad_kernel<<<(unsigned)grid, 256, 0, (hipStream_t)stream>>>(p);
+    p.tiles_n = pl.tiles_n; p.tiles_k = pl.tiles_k; p.splits = pl.splits; p.tiles_per_split = pl.per;
+    if (pl.big) mx_wgrad_kernel<128, 256, 64, 64><<<(unsigned)grid, 512, 0, s>>>(p);
+    else mx_wgrad_kernel<64, 64, 32, 32><<<(unsigned)grid, 256, 0, s>>>(p);
+    if (pl.splits > 1) {
+        const int64_t quads = (nk > n_out ? nk : n_out) / 4 + 1;
+        mx_wgrad_join_kernel<<<(unsigned)((quads + 255) / 256), 256, 0, s>>>(pw, pb, dW, dbias, nk, n_out, pl.splits, nk % 4 == 0);
+    }
     return check_launch("swat_mx_linear_wgrad");
 }
