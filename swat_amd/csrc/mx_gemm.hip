@@ -6,6 +6,8 @@
 // the fp32 accumulator.  e2m1 by e2m1 loses nothing by it (multiples of 1/4 up to 36); with an e4m3 operand up to 2^-13 of the largest
 // product can go, which a bfloat16 result does not show and a float32 one would: those products come out in bfloat16 only.  Lane (r = lane & 15, g = lane >> 4) feeds row r; e2m1: columns 32 g .. + 31 (16 bytes);
 // e4m3: columns 16 g .. + 15 and 64 + 16 g .. + 15; its scale operand is the byte of block g of the 128 columns in both.
+#include <math.h>
+#include <type_traits>
 #include "gemm_device.hpp"
 #include "mx_device.hpp"
 #include "../../include/swat_hip.h"
@@ -13,6 +15,7 @@
 namespace swat {
 
 typedef int mx_v8i __attribute__((ext_vector_type(8)));
+typedef unsigned mx_u4 __attribute__((ext_vector_type(4)));
 
 struct MxGemmArgs {
     const unsigned char *A, *B, *sA, *sB;
@@ -21,30 +24,18 @@ struct MxGemmArgs {
     int64_t M, N;
     int blocks, out_bf;   // blocks of 32 along k
     int tiles_m, tiles_n;
+    int m_begin;          // first row of this launch
 };
 
-__device__ const uint4 mx_zero_chunk = {0u, 0u, 0u, 0u};   // what lanes past the last row or column load
-
 template <int BITS>
-__device__ __forceinline__ int mx_lds_off(int row, int c) {  // 16-byte chunk c of a row of 128 packed columns
+__device__ __forceinline__ constexpr int mx_lds_off(int row, int c) {  // 16-byte chunk c of a row of 128 packed columns
     if constexpr (BITS == 4) return row * 64 + ((c ^ ((row >> 2) & 3)) << 4);
     else return row * 128 + ((c ^ ((row >> 1) & 7)) << 4);
 }
-template <int BITS>
-__device__ __forceinline__ mx_v8i mx_frag(const unsigned char* tile, int row, int g) {
-    mx_v8i v = {0, 0, 0, 0, 0, 0, 0, 0};
-    const uint4 lo = *reinterpret_cast<const uint4*>(tile + mx_lds_off<BITS>(row, g));
-    v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w;
-    if constexpr (BITS == 8) {
-        const uint4 hi = *reinterpret_cast<const uint4*>(tile + mx_lds_off<8>(row, 4 + g));
-        v[4] = hi.x; v[5] = hi.y; v[6] = hi.z; v[7] = hi.w;
-    }
-    return v;
-}
-// D[n][m] += B[n] . A[m]
-template <int AB, int BB>
+// D[n][m] += B[n] . A[m]; the scales are byte S of sb, sa
+template <int AB, int BB, int S>
 __device__ __forceinline__ f32x4_t mx_mfma(mx_v8i b, mx_v8i a, f32x4_t c, int sb, int sa) {
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, a, c, BB == 4 ? 4 : 0, AB == 4 ? 4 : 0, 0, sb, 0, sa);
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, a, c, BB == 4 ? 4 : 0, AB == 4 ? 4 : 0, S, sb, S, sa);
 }
 
 // lane holds C[m][n .. n + 3]
@@ -69,57 +60,364 @@ __device__ __forceinline__ void mx_store4(const MxGemmArgs& p, int64_t m, int64_
         }
 }
 
-template <int AB, int BB>
-__global__ __launch_bounds__(256) void mx_gemm_kernel(MxGemmArgs p) {
-    constexpr int BM = 128, BN = 128, RA = 16 * AB, RB = 16 * BB;
-    __shared__ __attribute__((aligned(1024))) unsigned char smem[BM * RA + BN * RB];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int r16 = lane & 15, g = lane >> 4, wr = wave >> 1, wc = wave & 1;
-    const int64_t m0 = (int64_t)(blockIdx.x % p.tiles_m) * BM, n0 = (int64_t)(blockIdx.x / p.tiles_m) * BN;
-    const int64_t rowA = (int64_t)p.blocks * 4 * AB, rowB = (int64_t)p.blocks * 4 * BB;  // bytes of a packed row
-    f32x4_t acc[4][4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
-    const int nk = (p.blocks + 3) / 4;
-    for (int kt = 0; kt < nk; ++kt) {
-        __syncthreads();
-        for (int i = tid; i < BM * RA / 16; i += 256) {
-            const int row = i / (RA / 16), c = i % (RA / 16);
-            const int64_t m = m0 + row, at = (int64_t)kt * RA + c * 16;
-            const uint4 v = m < p.M && at < rowA ? *reinterpret_cast<const uint4*>(p.A + m * rowA + at) : mx_zero_chunk;
-            *reinterpret_cast<uint4*>(smem + mx_lds_off<AB>(row, c)) = v;
-        }
-        for (int i = tid; i < BN * RB / 16; i += 256) {
-            const int row = i / (RB / 16), c = i % (RB / 16);
-            const int64_t n = n0 + row, at = (int64_t)kt * RB + c * 16;
-            const uint4 v = n < p.N && at < rowB ? *reinterpret_cast<const uint4*>(p.B + n * rowB + at) : mx_zero_chunk;
-            *reinterpret_cast<uint4*>(smem + BM * RA + mx_lds_off<BB>(row, c)) = v;
-        }
-        __syncthreads();
-        mx_v8i fb[4];
-        int sb[4];
-        const int kb = 4 * kt + g;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int row = 64 * wc + 16 * j + r16;
-            fb[j] = mx_frag<BB>(smem + BM * RA, row, g);
-            sb[j] = n0 + row < p.N && kb < p.blocks ? p.sB[(n0 + row) * p.blocks + kb] : 0;
-        }
+// 16 scale bytes of a row from block `first` on, blocks past the row's end as zeros.  Rows sit on any byte: where 16 bytes would reach past
+// the matrix's end the load is moved back and its bytes shifted down (the matrix has 16 bytes at least).
+__device__ __forceinline__ mx_u4 mx_scales16(const unsigned char* s, int64_t at, int64_t total) {
+    const int64_t to = at + 16 <= total ? at : total - 16;
+    mx_u4 v;
+    __builtin_memcpy(&v, s + to, 16);
+    const int sh = at - to < 16 ? (int)(at - to) : 16;
+    if (sh) {
+        unsigned w[9] = {v[0], v[1], v[2], v[3], 0u, 0u, 0u, 0u, 0u};
+        const int d = sh >> 2, b = (sh & 3) * 8;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int row = 64 * wr + 16 * i + r16;
-            const mx_v8i fa = mx_frag<AB>(smem, row, g);
-            const int sa = m0 + row < p.M && kb < p.blocks ? p.sA[(m0 + row) * p.blocks + kb] : 0;
+            unsigned lo = 0u, hi = 0u;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[i][j] = mx_mfma<AB, BB>(fb[j], fa, acc[i][j], sb[j], sa);
+            for (int j = 0; j < 5; ++j) {
+                lo = d == j ? w[i + j] : lo;
+                hi = d == j ? w[i + j + 1 < 9 ? i + j + 1 : 8] : hi;
+            }
+            v[i] = b ? lo >> b | hi << (32 - b) : lo;
         }
     }
+    return v;
+}
+
+// A workgroup computes BM x BN of C in waves of WM x WN.  Bound by the matrix cores and by the bytes a CU can load where it is large (256 x 256 in
+// 8 waves of 128 x 64: 16448 x 1024 x 4096 in 4 bits 54 us, 2.6 PFLOP/s, 8192^3 325 us, 3.4; the matrix instructions alone 29 of the
+// first's 45 us: all CUs at once run them at a lower clock than a few).  128 columns at a time: codes go through registers into one of two LDS buffers while
+// the matrix cores work on the other, loads two tiles ahead.  A row's scales come 16 bytes (four tiles) at a time, are transposed to
+// [block of the tile][tile] and kept in LDS, so that one 4-byte read gives a lane the scales of its row and block for four tiles, which
+// the instruction picks by byte.
+template <int AB, int BB, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, 2) void mx_gemm_kernel(MxGemmArgs p) {
+    constexpr int NT = (BM / WM) * (BN / WN) * 64, FM = WM / 16, FN = WN / 16;
+    constexpr int RA = 16 * AB, RB = 16 * BB, CRA = RA / 16, CRB = RB / 16;          // bytes, chunks of a tile's row
+    constexpr int CA = BM * CRA / NT, CB = BN * CRB / NT, RSA = NT / CRA, RSB = NT / CRB;   // chunks to a thread and the rows between them
+    constexpr int BUF = BM * RA + BN * RB, ROWS = BM + BN;
+    static_assert(CA * NT == BM * CRA && CB * NT == BN * CRB && RSA % 16 == 0 && RSB % 16 == 0 && ROWS <= 2 * NT, "whole chunks");
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * BUF + 2 * ROWS * 16];
+    unsigned char* const ssc = smem + 2 * BUF;   // scales: [2][A rows | B rows][block of the tile][tile of four]
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int r16 = lane & 15, g = lane >> 4, wr = wave / (BN / WN), wc = wave % (BN / WN);
+    // units of one XCD (workgroups b, b + 8, ..) are neighbours, 4 column tiles wide: its L2 sees few panels of either operand
+    int id;
+    {
+        const int total = gridDim.x, xcd = blockIdx.x & 7, q = total >> 3, r = total & 7;
+        id = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (blockIdx.x >> 3);
+    }
+    const int band = id / (4 * p.tiles_m), wide = p.tiles_n - 4 * band < 4 ? p.tiles_n - 4 * band : 4;
+    const int tn = 4 * band + (id - 4 * band * p.tiles_m) % wide, tm = (id - 4 * band * p.tiles_m) / wide;
+    const int64_t m0 = p.m_begin + (int64_t)tm * BM, n0 = (int64_t)tn * BN;
+    const int rowA = p.blocks * 4 * AB, rowB = p.blocks * 4 * BB;   // bytes of a packed row
+    const int nk = (p.blocks + 3) / 4;
+
+    // codes: buffer descriptors that start at the tile's rows and end with the matrix (rows past it read as zeros), advanced along k;
+    // chunks past a row's end get an offset past the end
+    constexpr unsigned OUT = 0x80000000u;
+    const int rowsA = p.M - m0 < BM ? (int)(p.M - m0) : BM, rowsB = p.N - n0 < BN ? (int)(p.N - n0) : BN;
+    const unsigned char *ga = p.A + m0 * rowA, *gb = p.B + n0 * rowB;
+    int left = 4 * p.blocks * 4;   // 4-bit bytes of a row still to load: AB / 4 times that of A
+    const int ra = tid / CRA, ca = tid % CRA, rb = tid / CRB, cb = tid % CRB;
+    const unsigned oa = (unsigned)(ra * rowA + ca * 16), ob = (unsigned)(rb * rowB + cb * 16);
+    unsigned char *const wa = smem + mx_lds_off<AB>(ra, ca), *const wb = smem + BM * RA + mx_lds_off<BB>(rb, cb);
+    struct Stage {
+        mx_u4 a[CA], b[CB];
+    };
+    constexpr bool DEEP = WM * WN <= 4096 && AB + BB < 16;   // two tiles of loads in flight; one where the registers do not reach
+    Stage st0, st1_;
+    Stage& st1 = DEEP ? st1_ : st0;
+    auto load = [&](Stage& st) {
+        const int la = left * (AB / 4), lb = left * (BB / 4);   // (<= 0: past the last tile)
+        const __amdgpu_buffer_rsrc_t da = __builtin_amdgcn_make_buffer_rsrc((void*)ga, 0, la > 0 ? (rowsA - 1) * rowA + la : 0, 0x20000);
+        const __amdgpu_buffer_rsrc_t db = __builtin_amdgcn_make_buffer_rsrc((void*)gb, 0, lb > 0 ? (rowsB - 1) * rowB + lb : 0, 0x20000);
+        const unsigned pa = ca * 16 < la ? oa : OUT, pb = cb * 16 < lb ? ob : OUT;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < CA; ++i) st.a[i] = __builtin_amdgcn_raw_buffer_load_b128(da, pa + (unsigned)(i * RSA * rowA), 0, 0);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) mx_store4(p, m0 + 64 * wr + 16 * i + r16, n0 + 64 * wc + 16 * j + 4 * g, acc[i][j]);
+        for (int i = 0; i < CB; ++i) st.b[i] = __builtin_amdgcn_raw_buffer_load_b128(db, pb + (unsigned)(i * RSB * rowB), 0, 0);
+        ga += RA;
+        gb += RB;
+        left -= 64;
+    };
+    auto put = [&](const Stage& st, int buf) {
+#pragma unroll
+        for (int i = 0; i < CA; ++i) *reinterpret_cast<mx_u4*>(wa + buf * BUF + i * RSA * RA) = st.a[i];
+#pragma unroll
+        for (int i = 0; i < CB; ++i) *reinterpret_cast<mx_u4*>(wb + buf * BUF + i * RSB * RB) = st.b[i];
+    };
+    // scales: a thread takes one or two rows of the tile
+    constexpr int SR = (ROWS + NT - 1) / NT;
+    mx_u4 sc[SR];
+    int s_next = 0;   // next group of four tiles to load
+    auto load_scales = [&]() {
+#pragma unroll
+        for (int i = 0; i < SR; ++i) {
+            const int r = tid + i * NT;
+            const bool isa = r < BM;
+            int64_t row = isa ? m0 + r : n0 + (r - BM);
+            const int64_t most = isa ? p.M : p.N;
+            row = row < most ? row : most - 1;   // (rows past the matrix: any scale, their codes are zeros)
+            const int first = 16 * s_next < p.blocks ? 16 * s_next : 0;
+            sc[i] = mx_scales16(isa ? p.sA : p.sB, row * p.blocks + first, most * p.blocks);
+        }
+    };
+    auto put_scales = [&](int buf) {
+        const int have = p.blocks - 16 * s_next;   // blocks of this group inside the row; the rest gets scale byte 0 (zeros times 2^-127)
+#pragma unroll
+        for (int i = 0; i < SR; ++i) {
+            const int r = tid + i * NT;
+            if (ROWS % NT && r >= ROWS) break;
+            unsigned w[4];
+#pragma unroll
+            for (int d = 0; d < 4; ++d) w[d] = have >= 4 * d + 4 ? sc[i][d] : have <= 4 * d ? 0u : sc[i][d] & ((1u << 8 * (have - 4 * d)) - 1u);
+            // bytes [tile][block] -> [block][tile]
+            const unsigned p0 = __builtin_amdgcn_perm(w[1], w[0], 0x05010400), p1 = __builtin_amdgcn_perm(w[1], w[0], 0x07030602);
+            const unsigned q0 = __builtin_amdgcn_perm(w[3], w[2], 0x05010400), q1 = __builtin_amdgcn_perm(w[3], w[2], 0x07030602);
+            const mx_u4 t = {__builtin_amdgcn_perm(q0, p0, 0x05040100), __builtin_amdgcn_perm(q0, p0, 0x07060302),
+                             __builtin_amdgcn_perm(q1, p1, 0x05040100), __builtin_amdgcn_perm(q1, p1, 0x07060302)};
+            *reinterpret_cast<mx_u4*>(ssc + (buf * ROWS + r) * 16) = t;
+        }
+        ++s_next;
+    };
+    auto bar = [&]() {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+
+    f32x4_t acc[FM][FN];
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+    int sa[FM], sb[FN];
+    auto read_scales = [&](int buf) {
+        const unsigned char* q = ssc + buf * ROWS * 16 + 4 * g;
+#pragma unroll
+        for (int i = 0; i < FM; ++i) sa[i] = *reinterpret_cast<const int*>(q + (WM * wr + 16 * i + r16) * 16);
+#pragma unroll
+        for (int j = 0; j < FN; ++j) sb[j] = *reinterpret_cast<const int*>(q + (BM + WN * wc + 16 * j + r16) * 16);
+    };
+    // (fragment rows are 16 apart: the chunk permutation depends on r16 alone)
+    const unsigned char* const pa0 = smem + WM * wr * RA + mx_lds_off<AB>(r16, g);
+    const unsigned char* const pa1 = smem + WM * wr * RA + mx_lds_off<AB>(r16, AB == 8 ? 4 + g : g);
+    const unsigned char* const pb0 = smem + BM * RA + WN * wc * RB + mx_lds_off<BB>(r16, g);
+    const unsigned char* const pb1 = smem + BM * RA + WN * wc * RB + mx_lds_off<BB>(r16, BB == 8 ? 4 + g : g);
+    auto frag = [&](const unsigned char* lo, const unsigned char* hi, auto bits) {
+        const mx_u4 l = *reinterpret_cast<const mx_u4*>(lo);
+        mx_v8i v = {(int)l[0], (int)l[1], (int)l[2], (int)l[3], 0, 0, 0, 0};
+        if constexpr (decltype(bits)::value == 8) {
+            const mx_u4 h = *reinterpret_cast<const mx_u4*>(hi);
+            v[4] = (int)h[0]; v[5] = (int)h[1]; v[6] = (int)h[2]; v[7] = (int)h[3];
+        }
+        return v;
+    };
+    auto multiply = [&](int buf, auto tile) {
+        constexpr int S = decltype(tile)::value;
+        mx_v8i fb[FN];
+#pragma unroll
+        for (int j = 0; j < FN; ++j) fb[j] = frag(pb0 + buf * BUF + 16 * j * RB, pb1 + buf * BUF + 16 * j * RB, std::integral_constant<int, BB>{});
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+            const mx_v8i fa = frag(pa0 + buf * BUF + 16 * i * RA, pa1 + buf * BUF + 16 * i * RA, std::integral_constant<int, AB>{});
+#pragma unroll
+            for (int j = 0; j < FN; ++j) acc[i][j] = mx_mfma<AB, BB, S>(fb[j], fa, acc[i][j], sb[j], sa[i]);
+        }
+    };
+
+    load_scales();
+    load(st0);
+    if constexpr (DEEP) load(st1);
+    put_scales(0);
+    load_scales();
+    put(st0, 0);
+    load(st0);
+    bar();
+    int t = 0;
+    for (int sbuf = 0;; sbuf ^= 1) {
+        read_scales(sbuf);
+        put(st1, 1);
+        load(st1);
+        multiply(0, std::integral_constant<int, 0>{});
+        bar();
+        if (++t >= nk) break;
+        put(st0, 0);
+        load(st0);
+        multiply(1, std::integral_constant<int, 1>{});
+        bar();
+        if (++t >= nk) break;
+        put(st1, 1);
+        load(st1);
+        put_scales(sbuf ^ 1);   // (read last two tiles ago)
+        load_scales();
+        multiply(0, std::integral_constant<int, 2>{});
+        bar();
+        if (++t >= nk) break;
+        put(st0, 0);
+        load(st0);
+        multiply(1, std::integral_constant<int, 3>{});
+        bar();
+        if (++t >= nk) break;
+    }
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) mx_store4(p, m0 + WM * wr + 16 * i + r16, n0 + WN * wc + 16 * j + 4 * g, acc[i][j]);
+}
+
+// Few rows: a workgroup computes 16 columns of 16 FM rows, its 8 waves take the 128-column tiles of k in turn, straight from memory into
+// registers (nothing is used twice), and their sums meet in LDS in the order of the waves.  Bound by latency and B's bytes.  Addresses past
+// an edge are moved to readable ones and what they load is replaced by zeros, so that all loads of several tiles go out together.
+template <int AB, int BB, int FM>
+__global__ __launch_bounds__(512, 2) void mx_rows_kernel(MxGemmArgs p) {
+    __shared__ f32x4_t part[8][FM][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, g = lane >> 4;
+    p.m_begin += (int)blockIdx.x / p.tiles_n * (16 * FM);
+    const int64_t n0 = (int64_t)((int)blockIdx.x % p.tiles_n) * 16, n = n0 + r16;
+    const int64_t rowA = (int64_t)p.blocks * 4 * AB, rowB = (int64_t)p.blocks * 4 * BB;
+    f32x4_t acc[FM];
+#pragma unroll
+    for (int i = 0; i < FM; ++i) acc[i] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+    auto piece = [&](const unsigned char* row, int at, bool live) {
+        mx_u4 v = *reinterpret_cast<const mx_u4*>(row + (live ? at : 0));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = live ? v[e] : 0u;
+        return v;
+    };
+    auto frag = [&](const unsigned char* row, int kt, bool live, auto bits) {
+        constexpr int BITS = decltype(bits)::value;
+        mx_v8i v = {0, 0, 0, 0, 0, 0, 0, 0};
+        if constexpr (BITS == 4) {
+            const mx_u4 l = piece(row, 64 * kt + 16 * g, live && 4 * kt + g < p.blocks);
+            v[0] = (int)l[0]; v[1] = (int)l[1]; v[2] = (int)l[2]; v[3] = (int)l[3];
+        } else {   // columns 16 g .. and 64 + 16 g ..: half a block each
+            const mx_u4 l = piece(row, 128 * kt + 16 * g, live && 4 * kt + g / 2 < p.blocks);
+            const mx_u4 h = piece(row, 128 * kt + 64 + 16 * g, live && 4 * kt + 2 + g / 2 < p.blocks);
+            v[0] = (int)l[0]; v[1] = (int)l[1]; v[2] = (int)l[2]; v[3] = (int)l[3];
+            v[4] = (int)h[0]; v[5] = (int)h[1]; v[6] = (int)h[2]; v[7] = (int)h[3];
+        }
+        return v;
+    };
+    const int nk = (p.blocks + 3) / 4;
+    const bool live_n = n < p.N;
+    const int64_t nn = live_n ? n : n0;
+    const unsigned char *bp = p.B + nn * rowB, *bs = p.sB + nn * p.blocks;
+    const unsigned char *ap[FM], *as[FM];
+    bool live_m[FM];
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+        const int64_t m = p.m_begin + 16 * i + r16;
+        live_m[i] = m < p.M;
+        const int64_t mm = live_m[i] ? m : p.m_begin;
+        ap[i] = p.A + mm * rowA;
+        as[i] = p.sA + mm * p.blocks;
+    }
+    auto tiles = [&](int kt0, auto count) {   // `count` tiles of k, 8 apart: loads first, then the products in order
+        constexpr int C = decltype(count)::value;
+        mx_v8i fb[C], fa[C][FM];
+        int sb[C], sa[C][FM];
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int kt = kt0 + 8 * c;
+            const bool inside = 4 * kt + g < p.blocks;
+            const int ks = inside ? 4 * kt + g : 0;
+            fb[c] = frag(bp, kt, live_n, std::integral_constant<int, BB>{});
+            sb[c] = bs[ks];
+#pragma unroll
+            for (int i = 0; i < FM; ++i) {
+                fa[c][i] = frag(ap[i], kt, live_m[i], std::integral_constant<int, AB>{});
+                sa[c][i] = as[i][ks];
+            }
+            sb[c] = inside ? sb[c] : 0;
+#pragma unroll
+            for (int i = 0; i < FM; ++i) sa[c][i] = inside ? sa[c][i] : 0;
+        }
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int i = 0; i < FM; ++i) acc[i] = mx_mfma<AB, BB, 0>(fb[c], fa[c][i], acc[i], sb[c], sa[c][i]);
+    };
+    int kt = wave;
+    constexpr int AHEAD = FM == 4 && AB + BB > 8 ? 2 : 4;
+    for (; kt + 8 * (AHEAD - 1) < nk; kt += 8 * AHEAD) tiles(kt, std::integral_constant<int, AHEAD>{});
+    for (; kt < nk; kt += 8) tiles(kt, std::integral_constant<int, 1>{});
+#pragma unroll
+    for (int i = 0; i < FM; ++i) part[wave][i][lane] = acc[i];
+    __syncthreads();
+    if (wave < FM) {
+        f32x4_t s = part[0][wave][lane];
+#pragma unroll
+        for (int w = 1; w < 8; ++w) s += part[w][wave][lane];
+        mx_store4(p, p.m_begin + 16 * wave + r16, n0 + 4 * g, s);
+    }
+}
+
+template <int AB, int BB>
+static void mx_rows(MxGemmArgs p, int64_t m_begin, int rows, hipStream_t s) {
+    // a workgroup to each 16-row part while they stay within 2 to a CU (64 rows, 4 bits, k 4096: 1024 columns 5.7 us with 256 workgroups,
+    // 10.9 with 64; k 1024: 4096 columns 5.8 with 1024, 4.8 with 256)
+    p.m_begin = (int)m_begin;
+    p.tiles_n = (int)((p.N + 15) / 16);
+    const int parts = (rows + 15) / 16;
+    if ((int64_t)p.tiles_n * parts <= 512) mx_rows_kernel<AB, BB, 1><<<(unsigned)(p.tiles_n * parts), 512, 0, s>>>(p);
+    else mx_rows_kernel<AB, BB, 4><<<(unsigned)(p.tiles_n * ((parts + 3) / 4)), 512, 0, s>>>(p);
+}
+template <int AB, int BB, int BM, int BN, int WM, int WN>
+static void mx_tiles(MxGemmArgs p, int64_t rows, hipStream_t s) {
+    p.M = rows;   // (rows behind them, if any, go to mx_rows)
+    p.tiles_m = (int)((rows + BM - 1) / BM);
+    p.tiles_n = (int)((p.N + BN - 1) / BN);
+    mx_gemm_kernel<AB, BB, BM, BN, WM, WN><<<(unsigned)(p.tiles_m * p.tiles_n), (BM / WM) * (BN / WN) * 64, 0, s>>>(p);
+}
+
+// Which tile, by the sum of what was measured (us, 4 by 4 bits; an 8-bit operand adds 28 %): a 128-column step takes a CU 0.8 with five
+// 64 x 64 workgroups on it (0.25 with one), 0.78 with two of 128 x 128 (0.45 with one), 1.2 with one of 256 x 256; a round of workgroups
+// 2.5, 3.5, 7 more (the last is alone on its CU while it stores).  Up to 64 rows past whole tiles may go to mx_rows (5) instead of a round of
+// their own.  Few rows and columns: mx_rows.
+//   4 x 4 bits, 64 x 64 / 128 x 128 / 256 x 256: 1600 x 768 x 768 5.9 / 7.5 / 15.8; 8239 x 2048 x 1000 35 / 28.1 / 37.8 (25.9 with the last rows
+//   apart); 16448 x 1024 x 4096 110 / 68 / 87 (53.9); 8192^3 795 / 416 / 325.   64 rows, 1024 x 4096 5.7 in mx_rows, 11.1 in 64 x 64;
+//   64 rows, 65536 x 512 20 and 8.2
+struct MxGemmPlan {
+    int size;        // 0: mx_rows, 1: 64 x 64, 2: 128 x 128, 3: 256 x 256
+    int64_t rows;    // those of the tile kernel; what is behind goes to mx_rows
+};
+static MxGemmPlan mx_plan(int64_t M, int64_t N, int blocks, int ab, int bb) {
+    const int64_t cols16 = (N + 15) / 16;
+    // (fewer than 16 scale bytes in an operand: the tile kernels load them by 16)
+    if ((M <= 64 && cols16 <= 512) || M * blocks < 16 || N * blocks < 16) return {0, 0};
+    static const double full[4] = {0, 0.8, 0.78, 1.2}, alone[4] = {0, 0.25, 0.45, 1.2}, round[4] = {0, 2.5, 3.5, 7.0};
+    static const int slots[4] = {0, 5, 2, 1};
+    const double f = 1.0 + 0.07 * (ab + bb - 8), steps = (blocks + 3) / 4;
+    MxGemmPlan best = {};
+    double cost = -1;
+    for (int size = 1; size <= 3; ++size) {
+        const int b = 32 << size;
+        const int64_t tn = (N + b - 1) / b, rem = M % b;
+        for (int tail = 0; tail < 2; ++tail) {
+            if (tail && !(rem > 0 && rem <= 64 && M > b && size > 1)) continue;
+            const double tiles = (double)tn * (tail ? M / b : (M + b - 1) / b), per = 256.0 * slots[size];
+            const double whole = floor(tiles / per), rest = ceil((tiles - whole * per) / 256.0);   // workgroups to a CU in the last round
+            const double one = slots[size] > 1 ? (full[size] - alone[size]) / (slots[size] - 1) : 0.0;
+            double c = 4.0 + whole * (steps * full[size] * f + round[size]);
+            if (rest > 0) c += steps * (slots[size] > 1 ? alone[size] + (rest - 1) * one : full[size]) * f + round[size];
+            if (tail) c += 5.0;
+            if (cost < 0 || c < cost) {
+                cost = c;
+                best = {size, tail ? M - rem : M};
+            }
+        }
+    }
+    return best;
+}
+template <int AB, int BB>
+static void mx_product(const MxGemmArgs& p, hipStream_t s) {
+    const MxGemmPlan pl = mx_plan(p.M, p.N, p.blocks, AB, BB);
+    if (pl.size == 1) mx_tiles<AB, BB, 64, 64, 32, 32>(p, pl.rows, s);
+    else if (pl.size == 2) mx_tiles<AB, BB, 128, 128, 64, 64>(p, pl.rows, s);
+    else if (pl.size == 3) mx_tiles<AB, BB, 256, 256, 128, 64>(p, pl.rows, s);
+    for (int64_t m = pl.rows; m < p.M; m += 64) mx_rows<AB, BB>(p, m, p.M - m < 64 ? (int)(p.M - m) : 64, s);
 }
 
 }  // namespace swat
@@ -129,7 +427,7 @@ using namespace swat;
 SWAT_API int swat_mx_matmul(const void* a_codes, const void* a_scales, int a_bits, const void* b_codes, const void* b_scales, int b_bits,
                             const float* bias, void* c, int c_dtype, int64_t M, int64_t N, int K, swat_stream_t stream) {
     SWAT_REQUIRE((a_bits == 4 || a_bits == 8) && (b_bits == 4 || b_bits == 8), "swat_mx_matmul: %d and %d bits (4 or 8 each)", a_bits, b_bits);
-    SWAT_REQUIRE(M >= 0 && N >= 0 && K >= 1 && K <= (1 << 24) && M < (1ll << 31) && N < (1ll << 31), "swat_mx_matmul: %lld x %lld x %d", (long long)M, (long long)N, K);
+    SWAT_REQUIRE(M >= 0 && N >= 0 && K >= 1 && K <= (1 << 22) && M < (1ll << 31) && N < (1ll << 31), "swat_mx_matmul: %lld x %lld x %d", (long long)M, (long long)N, K);
     SWAT_REQUIRE(c_dtype == SWAT_BF16 || (c_dtype == SWAT_F32 && a_bits == 4 && b_bits == 4), "swat_mx_matmul: output type %d of %d by %d bits (bf16; fp32 where both have 4 bits)", c_dtype, a_bits, b_bits);
     if (M == 0 || N == 0) return 0;
     SWAT_REQUIRE(a_codes && a_scales && b_codes && b_scales && c, "swat_mx_matmul: both operands and the output are needed");
@@ -137,13 +435,10 @@ SWAT_API int swat_mx_matmul(const void* a_codes, const void* a_scales, int a_bit
     MxGemmArgs p = {};
     p.A = (const unsigned char*)a_codes; p.sA = (const unsigned char*)a_scales; p.B = (const unsigned char*)b_codes; p.sB = (const unsigned char*)b_scales;
     p.bias = bias; p.C = c; p.M = M; p.N = N; p.blocks = (K + 31) / 32; p.out_bf = c_dtype == SWAT_BF16;
-    p.tiles_m = (int)((M + 127) / 128); p.tiles_n = (int)((N + 127) / 128);
-    const int64_t grid = (int64_t)p.tiles_m * p.tiles_n;
-    SWAT_REQUIRE(grid < (1ll << 31), "swat_mx_matmul: %lld x %lld is past one launch", (long long)M, (long long)N);
     const hipStream_t s = (hipStream_t)stream;
-    if (a_bits == 4 && b_bits == 4) mx_gemm_kernel<4, 4><<<(unsigned)grid, 256, 0, s>>>(p);
-    else if (a_bits == 8 && b_bits == 4) mx_gemm_kernel<8, 4><<<(unsigned)grid, 256, 0, s>>>(p);
-    else if (a_bits == 4 && b_bits == 8) mx_gemm_kernel<4, 8><<<(unsigned)grid, 256, 0, s>>>(p);
-    else mx_gemm_kernel<8, 8><<<(unsigned)grid, 256, 0, s>>>(p);
+    if (a_bits == 4 && b_bits == 4) mx_product<4, 4>(p, s);
+    else if (a_bits == 8 && b_bits == 4) mx_product<8, 4>(p, s);
+    else if (a_bits == 4 && b_bits == 8) mx_product<4, 8>(p, s);
+    else mx_product<8, 8>(p, s);
     return check_launch("swat_mx_matmul");
 }

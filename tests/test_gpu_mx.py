@@ -192,6 +192,13 @@ def test_product(abits, bbits, M, N, K):
         assert (got - ref).norm() <= 2.0 ** -8 * ref.norm()
 
 
+@pytest.mark.parametrize("abits,bbits", [(4, 4), (8, 4), (4, 8), (8, 8)])
+@pytest.mark.parametrize("M,N,K", [(5000, 4100, 130), (4136, 8192, 300), (5130, 3000, 480), (8224, 1024, 520), (3000, 3001, 700)])
+def test_product_of_every_tile_size(abits, bbits, M, N, K):
+    """Sizes that the kernel cuts into 64, 128 and 256 wide tiles, some with their last rows in a launch of their own."""
+    test_product(abits, bbits, M, N, K)
+
+
 def eights(x):
     """The largest magnitude of every eight neighbouring columns."""
     return torch.nn.functional.pad(x.abs(), (0, -x.shape[1] % 8)).view(x.shape[0], -1, 8).amax(-1)
