@@ -126,36 +126,35 @@ def ptr(t):
 
 def rows_ptr(t, what, dtypes, cols=None):
     """(device pointer, row stride) of a 2-D GPU tensor on the current device whose rows are contiguous and do not overlap."""
-    if not isinstance(t, torch.Tensor) or t.dim() != 2 or t.dtype not in dtypes or (cols is not None and t.shape[1] != cols):
-        got = f"{tuple(t.shape)} {t.dtype}" if isinstance(t, torch.Tensor) else repr(t)
-        raise SwatHipError(f"{what}: a 2-D tensor{'' if cols is None else f' of {cols} columns'} in "
-                           f"{' or '.join(str(d)[6:] for d in dtypes)} is wanted, got {got}")
-    on_device(t, what)
-    rows, n = t.shape
-    ld = t.stride(0) if rows > 1 else n
-    if (n > 1 and t.stride(1) != 1) or ld < n:
-        raise SwatHipError(f"{what}: rows have to be contiguous and apart, got strides {t.stride()}")
-    return t.data_ptr(), ld
+    if isinstance(t, torch.Tensor) and t.dim() == 2 and t.dtype in dtypes and t.is_cuda and t.get_device() == _current():
+        rows, n = t.shape
+        if cols is None or n == cols:
+            if t.is_contiguous():
+                return t.data_ptr(), n
+            ld = t.stride(0) if rows > 1 else n
+            if ld >= n and (n <= 1 or t.stride(1) == 1):
+                return t.data_ptr(), ld
+            raise SwatHipError(f"{what}: rows have to be contiguous and apart, got strides {t.stride()}")
+    got = f"{tuple(t.shape)} {t.dtype} on {t.device}" if isinstance(t, torch.Tensor) else repr(t)
+    raise SwatHipError(f"{what}: a 2-D GPU tensor{'' if cols is None else f' of {cols} columns'} in {' or '.join(str(d)[6:] for d in dtypes)} "
+                       f"on the current device is wanted (no CPU fallback), got {got}")
 
 
-def vec_ptr(t, what, n):
-    """Device pointer of a contiguous fp32 tensor of shape n (or None)."""
+def vec_ptr(t, what, *shape):
+    """Device pointer of a contiguous fp32 tensor of that shape on the current device (or None)."""
     if t is None:
         return None
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or tuple(t.shape) != n or not t.is_contiguous():
-        got = f"{tuple(t.shape)} {t.dtype}" if isinstance(t, torch.Tensor) else repr(t)
-        raise SwatHipError(f"{what}: a contiguous float32 tensor of shape {n} is wanted, got {got}")
-    on_device(t, what)
+    if not (isinstance(t, torch.Tensor) and t.dtype == torch.float32 and t.shape == shape and t.is_contiguous() and t.is_cuda
+            and t.get_device() == _current()):
+        got = f"{tuple(t.shape)} {t.dtype} on {t.device}" if isinstance(t, torch.Tensor) else repr(t)
+        raise SwatHipError(f"{what}: a contiguous float32 GPU tensor of shape {shape} on the current device is wanted (no CPU fallback), got {got}")
     return t.data_ptr()
 
 
-def on_device(t, what):
-    """Kernels launch on the current device's current stream: a tensor elsewhere is refused instead of read from there."""
-    if not t.is_cuda:
-        raise SwatHipError(f"{what}: swat_amd ops need GPU tensors (no CPU fallback)")
-    if t.device.index != torch.cuda.current_device():
-        raise SwatHipError(f"{what}: tensor on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+def _current():
+    """Kernels launch on the current device's current stream: a tensor on another device is refused instead of read from there."""
+    return torch._C._cuda_getDevice()
 
 
 def stream():
-    return torch.cuda.current_stream().cuda_stream
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())  # (current_stream().cuda_stream without the Stream object: 0.4 us, not 2.9)

@@ -7,7 +7,10 @@
 // backward pass reads that y.
 //
 // A row lives in the registers of one team of W waves; both norms take their mean and their squared deviations from there, so
-// every tensor crosses the memory bus once.  Bound by bytes in both directions.
+// every tensor crosses the memory bus once.  Rows may start on any element: vector loads and stores take any address here, and the last
+// columns of a width that is no multiple of 4 come as the row's last four, shifted down in registers.
+//
+// Bound by bytes in both directions (FIGURES).
 #include <type_traits>
 #include "kernels.hpp"
 #include "mx_device.hpp"
@@ -36,33 +39,106 @@ struct RnArgs {
     int rows, d, rows_per_team;
 };
 
-constexpr int RN_KINDS = 5;  // column sums of the backward pass: post_w, post_b, scale, pre_w, pre_b
+constexpr int RN_KINDS = 4;  // column sums of the backward pass: of gate gy hat, of gate gy, pre_w, pre_b
 
-template <int VEC>
-__device__ __forceinline__ void rn_load(const void* p, int bf, int64_t at, float (&v)[VEC]) {
-    if constexpr (VEC == 4) {
-        if (bf) {
-            const uint2 u = *reinterpret_cast<const uint2*>(reinterpret_cast<const unsigned short*>(p) + at);
-            v[0] = __uint_as_float(u.x << 16); v[1] = __uint_as_float(u.x & 0xffff0000u);
-            v[2] = __uint_as_float(u.y << 16); v[3] = __uint_as_float(u.y & 0xffff0000u);
-        } else {
-            const float4 f = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + at);
-            v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+typedef unsigned rn_u4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef unsigned rn_u2 __attribute__((ext_vector_type(2), aligned(2)));
+
+// Four neighbouring columns of a row, as they lie in memory.  T: 0 float32, 1 bfloat16, 2 by the flag.
+template <int T>
+struct RnRaw {
+    unsigned v[T == 1 ? 2 : 4];
+};
+template <int T>
+__device__ __forceinline__ void rn_raw(RnRaw<T>& r, const void* p, int bf, int64_t row, int c, int d) {
+    const int cc = c + 4 <= d || d < 4 ? c : d - 4;
+    const bool b = T == 1 || (T == 2 && bf);
+    if (d < 4) {   // (narrower than a vector: one lane, element by element)
+#pragma unroll
+        for (int e = 0; e < (T == 1 ? 2 : 4); ++e) r.v[e] = 0u;
+#pragma unroll
+        for (int e = 0; e < 3; ++e) {
+            if (e >= d) continue;
+            if (b) r.v[e >> 1] |= (unsigned)reinterpret_cast<const unsigned short*>(p)[row + e] << (16 * (e & 1));
+            else if constexpr (T != 1) r.v[e] = reinterpret_cast<const unsigned*>(p)[row + e];
         }
-    } else {
-        v[0] = bf ? bf2f(reinterpret_cast<const unsigned short*>(p)[at]) : reinterpret_cast<const float*>(p)[at];
+        return;
+    }
+    if (b) {
+        const rn_u2 u = *reinterpret_cast<const rn_u2*>(reinterpret_cast<const unsigned short*>(p) + row + cc);
+        r.v[0] = u[0];
+        r.v[1] = u[1];
+    } else if constexpr (T != 1) {
+        const rn_u4 u = *reinterpret_cast<const rn_u4*>(reinterpret_cast<const float*>(p) + row + cc);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r.v[e] = u[e];
     }
 }
-
-template <int VEC>
-__device__ __forceinline__ void rn_store(void* p, int bf, int64_t at, const float (&v)[VEC]) {
-    if constexpr (VEC == 4) {
-        if (bf) *reinterpret_cast<uint2*>(reinterpret_cast<unsigned short*>(p) + at) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
-        else *reinterpret_cast<float4*>(reinterpret_cast<float*>(p) + at) = make_float4(v[0], v[1], v[2], v[3]);
-    } else {
-        if (bf) reinterpret_cast<unsigned short*>(p)[at] = f2bf(v[0]);
-        else reinterpret_cast<float*>(p)[at] = v[0];
+// (columns past d: zeros)
+template <int T>
+__device__ __forceinline__ void rn_values(const RnRaw<T>& r, int bf, int c, int d, float (&v)[4]) {
+    if (T == 1 || (T == 2 && bf)) {
+        v[0] = __uint_as_float(r.v[0] << 16); v[1] = __uint_as_float(r.v[0] & 0xffff0000u);
+        v[2] = __uint_as_float(r.v[1] << 16); v[3] = __uint_as_float(r.v[1] & 0xffff0000u);
+    } else if constexpr (T != 1) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = __uint_as_float(r.v[e]);
     }
+    const int over = d & 3;   // columns of the last vector; it was loaded 4 - over columns early
+    if (over && d >= 4) {
+        const bool part = c < d && c + 4 > d;
+        if (over == 1) v[0] = part ? v[3] : v[0];
+        else if (over == 2) {
+            v[0] = part ? v[2] : v[0];
+            v[1] = part ? v[3] : v[1];
+        } else {
+            v[0] = part ? v[1] : v[0];
+            v[1] = part ? v[2] : v[1];
+            v[2] = part ? v[3] : v[2];
+        }
+#pragma unroll
+        for (int e = 1; e < 4; ++e) v[e] = part && e >= over ? 0.f : v[e];
+    }
+}
+__device__ __forceinline__ void rn_load(const void* p, int bf, int64_t row, int c, int d, float (&v)[4]) {
+    RnRaw<2> r;
+    rn_raw<2>(r, p, bf, row, c, d);
+    rn_values<2>(r, bf, c, d, v);
+}
+__device__ __forceinline__ void rn_load(const float* p, int64_t row, int c, int d, float (&v)[4]) {
+    RnRaw<0> r;
+    rn_raw<0>(r, p, 0, row, c, d);
+    rn_values<0>(r, 0, c, d, v);
+}
+__device__ __forceinline__ void rn_store(void* p, int bf, int64_t row, int c, int d, const float (&v)[4]) {
+    if (c + 4 <= d) {
+        if (bf) *reinterpret_cast<rn_u2*>(reinterpret_cast<unsigned short*>(p) + row + c) = (rn_u2){pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+        else *reinterpret_cast<rn_u4*>(reinterpret_cast<float*>(p) + row + c) =
+            (rn_u4){__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (c + e < d) {
+            if (bf) reinterpret_cast<unsigned short*>(p)[row + c + e] = f2bf(v[e]);
+            else reinterpret_cast<float*>(p)[row + c + e] = v[e];
+        }
+}
+
+// the wave's sum by lane shifts inside rows of 16 and two broadcasts of a row's last lane (a few cycles each; six LDS lane exchanges took
+// a tenth of the backward pass)
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp_add(float v) {
+    return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, true));
+}
+__device__ __forceinline__ float row_add_sum(float v) {
+    v = dpp_add<0x111, 0xf>(v);   // row_shr:1, 2, 4, 8
+    v = dpp_add<0x112, 0xf>(v);
+    v = dpp_add<0x114, 0xf>(v);
+    v = dpp_add<0x118, 0xf>(v);
+    v = dpp_add<0x142, 0xa>(v);   // row_bcast:15 into rows 1 and 3
+    v = dpp_add<0x143, 0xc>(v);   // row_bcast:31 into rows 2 and 3
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 
 // sums of N values over the team; sh: W * N floats of the team, two barriers around them (the trip count of the row loop is the
@@ -70,7 +146,7 @@ __device__ __forceinline__ void rn_store(void* p, int bf, int64_t at, const floa
 template <int W, int N>
 __device__ __forceinline__ void team_sum(float (&v)[N], float* sh) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = wave_sum(v[i]);
+    for (int i = 0; i < N; ++i) v[i] = row_add_sum(v[i]);
     if constexpr (W > 1) {
         const int wave = threadIdx.x >> 6;
         if ((threadIdx.x & 63) == 0) {
@@ -89,56 +165,62 @@ __device__ __forceinline__ void team_sum(float (&v)[N], float* sh) {
     }
 }
 
-// mean (layer) and 1 / deviation of a row held as v[NCH][VEC], columns c < d
-template <int W, int NCH, int VEC>
-__device__ __forceinline__ void row_stats(const float (&v)[NCH][VEC], int c0, int d, const RnArgs& a, float* sh, float& mean, float& rstd) {
+// mean (layer) and 1 / deviation of a row held as v[NCH][4], columns c < d
+template <int W, int NCH>
+__device__ __forceinline__ void row_stats(const float (&v)[NCH][4], int c0, int d, const RnArgs& a, float* sh, float& mean, float& rstd) {
     mean = 0.f;
     if (!a.rms) {
         float s[1] = {0.f};
 #pragma unroll
         for (int i = 0; i < NCH; ++i)
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) s[0] += v[i][e];  // (columns past d hold zeros)
+            for (int e = 0; e < 4; ++e) s[0] += v[i][e];  // (columns past d hold zeros)
         team_sum<W>(s, sh);
         mean = s[0] * a.inv_d;
     }
     float q[1] = {0.f};
 #pragma unroll
     for (int i = 0; i < NCH; ++i)
-        if (c0 + i * (64 * W * VEC) < d) {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                const float t = v[i][e] - mean;
-                q[0] = fmaf(t, t, q[0]);
-            }
+        for (int e = 0; e < 4; ++e) {
+            const float t = c0 + i * (256 * W) + e < d ? v[i][e] - mean : 0.f;
+            q[0] = fmaf(t, t, q[0]);
         }
     team_sum<W>(q, sh);
     rstd = 1.0f / sqrtf(q[0] * a.inv_d + a.eps);
 }
 
-// W waves to a row, NCH chunks of VEC columns to a lane: rows of up to 64 W NCH VEC columns
-template <int W, int NCH, int VEC>
+// W waves to a row, NCH vectors to a lane: rows of up to 256 W NCH columns
+template <int W, int NCH>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void residual_norm_fwd_kernel(RnArgs a) {
     __shared__ float sh[W];
     const int lane = threadIdx.x & (64 * W - 1);
     const int64_t row = W == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
     if (row >= a.rows) return;
-    const int d = a.d, c0 = lane * VEC;
-    constexpr int STEP = 64 * W * VEC;
-    float p[NCH][VEC], y[NCH][VEC];
+    const int d = a.d, c0 = lane * 4;
+    constexpr int STEP = 256 * W;
+    float p[NCH][4], y[NCH][4];
+    {
+        RnRaw<2> rh[NCH], rx[NCH];
 #pragma unroll
-    for (int i = 0; i < NCH; ++i) {
-        const int c = c0 + i * STEP;
+        for (int i = 0; i < NCH; ++i)
+            if (c0 + i * STEP < d) rn_raw<2>(rh[i], a.h, a.h_bf, row * a.sh, c0 + i * STEP, d);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) p[i][e] = y[i][e] = 0.f;
-        if (c < d) {
-            rn_load<VEC>(a.h, a.h_bf, row * a.sh + c, p[i]);
-            rn_load<VEC>(a.x, a.x_bf, row * a.sx + c, y[i]);
+        for (int i = 0; i < NCH; ++i)
+            if (c0 + i * STEP < d) rn_raw<2>(rx[i], a.x, a.x_bf, row * a.sx, c0 + i * STEP, d);
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) p[i][e] = y[i][e] = 0.f;
+            if (c0 + i * STEP < d) {
+                rn_values<2>(rh[i], a.h_bf, c0 + i * STEP, d, p[i]);
+                rn_values<2>(rx[i], a.x_bf, c0 + i * STEP, d, y[i]);
+            }
         }
     }
     float mean = 0.f, rstd = 1.f;
     if (a.post_w) {
-        row_stats<W, NCH, VEC>(p, c0, d, a, sh, mean, rstd);
+        row_stats<W, NCH>(p, c0, d, a, sh, mean, rstd);
         if (a.stats && lane == 0) {
             a.stats[row] = mean;
             a.stats[a.rows + row] = rstd;
@@ -150,35 +232,35 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void residual_norm_fwd_kerne
     for (int i = 0; i < NCH; ++i) {
         const int c = c0 + i * STEP;
         if (c >= d) continue;
-        float t[VEC], m[VEC];
+        float t[4], m[4];
         if (a.post_w) {
-            rn_load<VEC>(a.post_w, 0, c, t);
+            rn_load(a.post_w, 0, c, d, t);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) p[i][e] = (p[i][e] - mean) * rstd * t[e];
+            for (int e = 0; e < 4; ++e) p[i][e] = (p[i][e] - mean) * rstd * t[e];
             if (a.post_b) {
-                rn_load<VEC>(a.post_b, 0, c, t);
+                rn_load(a.post_b, 0, c, d, t);
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) p[i][e] += t[e];
+                for (int e = 0; e < 4; ++e) p[i][e] += t[e];
             }
         }
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) m[e] = g1;
-        if (a.gate_mode == 2) rn_load<VEC>(a.gate, 0, grp * d + c, m);
+        for (int e = 0; e < 4; ++e) m[e] = g1;
+        if (a.gate_mode == 2) rn_load(a.gate, grp * d, c, d, m);
         if (a.scale) {
-            rn_load<VEC>(a.scale, 0, c, t);
+            rn_load(a.scale, 0, c, d, t);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) m[e] *= t[e];
+            for (int e = 0; e < 4; ++e) m[e] *= t[e];
         }
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) y[i][e] = m[e] == 0.f ? a.alpha * y[i][e] : fmaf(a.alpha, y[i][e], m[e] * p[i][e]);
-        rn_store<VEC>(a.y, a.x_bf, row * d + c, y[i]);
+        for (int e = 0; e < 4; ++e) y[i][e] = c + e >= d ? 0.f : m[e] == 0.f ? a.alpha * y[i][e] : fmaf(a.alpha, y[i][e], m[e] * p[i][e]);
+        rn_store(a.y, a.x_bf, row * d, c, d, y[i]);
         if (a.x_bf) {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) y[i][e] = bf2f(f2bf(y[i][e]));  // the stream as stored
+            for (int e = 0; e < 4; ++e) y[i][e] = bf2f(f2bf(y[i][e]));  // the stream as stored
         }
     }
     if (!a.pre_w) return;
-    row_stats<W, NCH, VEC>(y, c0, d, a, sh, mean, rstd);
+    row_stats<W, NCH>(y, c0, d, a, sh, mean, rstd);
     if (a.stats && lane == 0) {
         a.stats[2 * (int64_t)a.rows + row] = mean;
         a.stats[3 * (int64_t)a.rows + row] = rstd;
@@ -186,39 +268,33 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void residual_norm_fwd_kerne
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
         const int c = c0 + i * STEP;
-        float z[VEC];
+        float z[4];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) z[e] = 0.f;
+        for (int e = 0; e < 4; ++e) z[e] = 0.f;
         if (c < d) {
-            float t[VEC];
-            rn_load<VEC>(a.pre_w, 0, c, t);
+            float t[4];
+            rn_load(a.pre_w, 0, c, d, t);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) z[e] = (y[i][e] - mean) * rstd * t[e];
+            for (int e = 0; e < 4; ++e) z[e] = (y[i][e] - mean) * rstd * t[e];
             if (a.pre_b) {
-                rn_load<VEC>(a.pre_b, 0, c, t);
+                rn_load(a.pre_b, 0, c, d, t);
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) z[e] += t[e];
+                for (int e = 0; e < 4; ++e) z[e] += t[e];
             }
-            if (a.z) rn_store<VEC>(a.z, a.z_bf, row * d + c, z);
+            if (a.z) rn_store(a.z, a.z_bf, row * d, c, d, z);
         }
-        if (a.z8) {  // blocks of 32 columns sit in 32 / VEC neighbouring lanes; the packed z is that of the z written beside it
-            if (a.z_bf) {
+        if (a.z8) {  // blocks of 32 columns sit in 8 neighbouring lanes; the packed z is that of the z written beside it
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) z[e] = bf2f(f2bf(z[e]));
-            }
+            for (int e = 0; e < 4; ++e) z[e] = c + e >= d ? 0.f : a.z_bf ? bf2f(f2bf(z[e])) : z[e];
             float top = 0.f;
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) top = mx_amax(top, z[e]);
+            for (int e = 0; e < 4; ++e) top = mx_amax(top, z[e]);
 #pragma unroll
-            for (int o = 1; o < 32 / VEC; o <<= 1) top = mx_amax(top, __shfl_xor(top, o, 64));
+            for (int o = 1; o < 8; o <<= 1) top = mx_amax(top, __shfl_xor(top, o, 64));
             const int sb = mx_scale_byte<8>(top);
             const float inv = mx_inverse(sb);
             if (c < a.z8_ld) {
-                if constexpr (VEC == 4) {
-                    *reinterpret_cast<unsigned*>(a.z8 + row * a.z8_ld + c) = sb == 255 ? 0x7f7f7f7fu : mx_e4m3x4(z[0] * inv, z[1] * inv, z[2] * inv, z[3] * inv);
-                } else {
-                    a.z8[row * a.z8_ld + c] = sb == 255 ? 0x7f : (unsigned char)(mx_e4m3x4(z[0] * inv, 0.f, 0.f, 0.f) & 0xff);
-                }
+                *reinterpret_cast<unsigned*>(a.z8 + row * a.z8_ld + c) = sb == 255 ? 0x7f7f7f7fu : mx_e4m3x4(z[0] * inv, z[1] * inv, z[2] * inv, z[3] * inv);
                 if (c % 32 == 0) a.z8s[row * a.z8s_ld + c / 32] = (unsigned char)sb;
             }
         }
@@ -228,116 +304,168 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void residual_norm_fwd_kerne
 // Backward.  With gy = dy + Norm_pre'(dz):  dx = alpha gy, and through y = alpha x + m p:
 //   dp = m gy (0 where m is), dh = Norm_post'(dp), d scale = sum_rows gate p gy, d gate = sum scale p gy over what shares it,
 //   Norm'(dn) = rstd (u - mean(u) - hat mean(u hat)), u = dn w  (rms: without mean(u)); d w = sum_rows dn hat, d b = sum_rows dn.
+// With A = sum_rows gate gy hat and B = sum_rows gate gy (p = hat w + b) the weights' gradients of the first norm and of the scale are
+// scale A, scale B and w A + b B: two column sums for three.
 // A team walks a contiguous range of rows and keeps the column sums of its lanes' columns in registers; the workgroup's teams meet
-// in LDS at the end, the workgroups in residual_norm_finish_kernel: a fixed order, no atomics.
-// (TEAMS teams to a workgroup: W == 1 only)
-template <int W, int NCH, int VEC, int TEAMS>
-__global__ __launch_bounds__(64 * W * TEAMS) void residual_norm_bwd_kernel(RnArgs a) {
-    constexpr int STEP = 64 * W * VEC, COLS = STEP * NCH;
-    __shared__ float sh[TEAMS > 1 ? TEAMS * COLS : 3 * W];
+// in LDS at the end, the workgroups in residual_norm_finish_kernel: a fixed order, no atomics.  The next row's four tensors are
+// loaded before the present row is worked on; the vectors of weights wait in LDS, so that nothing but those loads is in flight.
+// TEAMS teams to a workgroup (W == 1 only); TX, THZ: types of the stream and of h and dz (RnRaw; 2, 2: by the flags, no early loads);
+// GC: the gate is a row per group.
+template <int W, int NCH, int TEAMS, int TX, int THZ, bool GC>
+__global__ __launch_bounds__(64 * W * TEAMS, 2) void residual_norm_bwd_kernel(RnArgs a) {
+    constexpr int STEP = 256 * W, COLS = STEP * NCH, NT = 64 * W * TEAMS;
+    constexpr bool AHEAD = TX != 2 && !(GC && NCH > 3);   // (not where the registers do not reach)
+    __shared__ float red[3 * W];
+    __shared__ __attribute__((aligned(16))) float sh[(TEAMS > 4 ? TEAMS : 4) * COLS];   // pre_w, post_w, post_b, scale; at the end the teams' sums
     const int lane = threadIdx.x & (64 * W - 1), team_in = TEAMS > 1 ? threadIdx.x >> 6 : 0;
     const int64_t team = (int64_t)blockIdx.x * TEAMS + team_in;
-    const int d = a.d, c0 = lane * VEC;
+    const int d = a.d, c0 = lane * 4;
     const int64_t r0 = team * a.rows_per_team, r1 = r0 + a.rows_per_team < a.rows ? r0 + a.rows_per_team : a.rows;
-    float cs[RN_KINDS][NCH][VEC], cg[NCH][VEC];
+    for (int c = threadIdx.x; c < COLS; c += NT) {
+        sh[c] = a.pre_w && c < d ? a.pre_w[c] : 0.f;
+        sh[COLS + c] = c >= d ? 0.f : a.post_w ? a.post_w[c] : 1.f;
+        sh[2 * COLS + c] = a.post_b && c < d ? a.post_b[c] : 0.f;
+        sh[3 * COLS + c] = c >= d ? 0.f : a.scale ? a.scale[c] : 1.f;
+    }
+    __syncthreads();
+    auto vec = [&](int k, int i) { return *reinterpret_cast<const float4*>(sh + k * COLS + c0 + i * STEP); };
+    float cs[RN_KINDS][NCH][4], cg[GC ? 2 : 1][GC ? NCH : 1][4], gate[GC ? NCH : 1][4];   // cg: A and B of a group without its gate
 #pragma unroll
     for (int i = 0; i < NCH; ++i)
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
+        for (int e = 0; e < 4; ++e) {
 #pragma unroll
             for (int k = 0; k < RN_KINDS; ++k) cs[k][i][e] = 0.f;
-            cg[i][e] = 0.f;
+            if constexpr (GC) cg[0][i][e] = cg[1][i][e] = gate[i][e] = 0.f;
         }
-    int64_t grp = a.gate_mode && r0 < r1 ? r0 / a.rpg : 0, in_grp = a.gate_mode && r0 < r1 ? r0 - grp * a.rpg : 0;
+    struct Row {
+        RnRaw<TX> dy[NCH], y[NCH];
+        RnRaw<THZ> dz[NCH], h[NCH];
+        float st[4], g;
+    };
+    auto fetch = [&](Row& r, int64_t row) {
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            const int c = c0 + i * STEP;
+            if (c < d) {
+                rn_raw<THZ>(r.h[i], a.h, a.h_bf, row * a.sh, c, d);
+                if (a.dy) rn_raw<TX>(r.dy[i], a.dy, a.x_bf, row * a.sdy, c, d);
+                if (a.pre_w) {
+                    rn_raw<THZ>(r.dz[i], a.dz, a.z_bf, row * a.sdz, c, d);
+                    rn_raw<TX>(r.y[i], a.yin, a.x_bf, row * a.sy, c, d);
+                }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) r.st[k] = (k < 2 ? a.post_w != nullptr : a.pre_w != nullptr) ? a.stats[k * (int64_t)a.rows + row] : 0.f;
+        if constexpr (!GC) r.g = a.gate_mode == 1 ? a.gate[a.rpg == 1 ? row : row / a.rpg] : 1.f;
+    };
+    int64_t grp = 0, in_grp = 0;
+    if (a.gate_mode && r0 < r1) {
+        grp = r0 / a.rpg;
+        in_grp = r0 - grp * a.rpg;
+    }
+    auto load_gate = [&]() {
+        if constexpr (GC) {
+#pragma unroll
+            for (int i = 0; i < NCH; ++i)
+                if (c0 + i * STEP < d) rn_load(a.gate, grp * d, c0 + i * STEP, d, gate[i]);
+        }
+    };
+    Row next;
+    if (r0 < r1) {
+        if (AHEAD) fetch(next, r0);
+        load_gate();
+    }
     for (int64_t row = r0; row < r1; ++row) {
-        float gy[NCH][VEC], hv[NCH][VEC];
+        Row cur;
+        if constexpr (AHEAD) {
+            cur = next;
+            fetch(next, row + 1 < r1 ? row + 1 : row);
+        } else {
+            fetch(cur, row);
+        }
+        float gy[NCH][4], hv[NCH][4];
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
             const int c = c0 + i * STEP;
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) gy[i][e] = hv[i][e] = 0.f;
+            for (int e = 0; e < 4; ++e) gy[i][e] = hv[i][e] = 0.f;
             if (c < d) {
-                if (a.dy) rn_load<VEC>(a.dy, a.x_bf, row * a.sdy + c, gy[i]);
-                rn_load<VEC>(a.h, a.h_bf, row * a.sh + c, hv[i]);
+                if (a.dy) rn_values<TX>(cur.dy[i], a.x_bf, c, d, gy[i]);
+                rn_values<THZ>(cur.h[i], a.h_bf, c, d, hv[i]);
             }
         }
         if (a.pre_w) {
-            float u[NCH][VEC], hat[NCH][VEC];
-            const float mean = a.stats[2 * (int64_t)a.rows + row], rstd = a.stats[3 * (int64_t)a.rows + row];
+            float u[NCH][4], hat[NCH][4];
+            const float mean = cur.st[2], rstd = cur.st[3];
             float s[2] = {0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < NCH; ++i) {
                 const int c = c0 + i * STEP;
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) u[i][e] = hat[i][e] = 0.f;
-                if (c < d) {
-                    rn_load<VEC>(a.dz, a.z_bf, row * a.sdz + c, u[i]);
-                    rn_load<VEC>(a.yin, a.x_bf, row * a.sy + c, hat[i]);
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < NCH; ++i) {
-                const int c = c0 + i * STEP;
+                for (int e = 0; e < 4; ++e) u[i][e] = hat[i][e] = 0.f;
                 if (c >= d) continue;
-                float w[VEC];
-                rn_load<VEC>(a.pre_w, 0, c, w);
+                rn_values<THZ>(cur.dz[i], a.z_bf, c, d, u[i]);
+                rn_values<TX>(cur.y[i], a.x_bf, c, d, hat[i]);
+                const float4 w4 = vec(0, i);
+                const float w[4] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) {
+                for (int e = 0; e < 4; ++e) {
                     hat[i][e] = (hat[i][e] - mean) * rstd;
-                    cs[3][i][e] = fmaf(u[i][e], hat[i][e], cs[3][i][e]);
-                    cs[4][i][e] += u[i][e];
+                    cs[2][i][e] = fmaf(u[i][e], hat[i][e], cs[2][i][e]);
+                    cs[3][i][e] += u[i][e];
                     u[i][e] *= w[e];
                     s[0] += u[i][e];
-                    s[1] = fmaf(u[i][e], hat[i][e], s[1]);
+                    s[1] = fmaf(u[i][e], hat[i][e], s[1]);   // (columns past d: u is zero)
                 }
             }
-            team_sum<W>(s, sh);
+            team_sum<W>(s, red);
             const float m1 = a.rms ? 0.f : s[0] * a.inv_d, m2 = s[1] * a.inv_d;
 #pragma unroll
             for (int i = 0; i < NCH; ++i)
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) gy[i][e] = fmaf(rstd, u[i][e] - m1 - hat[i][e] * m2, gy[i][e]);
+                for (int e = 0; e < 4; ++e) gy[i][e] = fmaf(rstd, u[i][e] - m1 - hat[i][e] * m2, gy[i][e]);
         }
-        const float mean = a.post_w ? a.stats[row] : 0.f, rstd = a.post_w ? a.stats[(int64_t)a.rows + row] : 1.f;
-        const float g1 = a.gate_mode == 1 ? a.gate[grp] : 1.f;
+        const float mean = a.post_w ? cur.st[0] : 0.f, rstd = a.post_w ? cur.st[1] : 1.f;
         float s[3] = {0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
             const int c = c0 + i * STEP;
             if (c >= d) continue;
-            float t[VEC], w[VEC], b[VEC], g[VEC], sc[VEC], dp[VEC];
+            float t[4];
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
+            for (int e = 0; e < 4; ++e) {
+                gy[i][e] = c + e < d ? gy[i][e] : 0.f;
                 t[e] = a.alpha * gy[i][e];
-                w[e] = sc[e] = 1.f;
-                b[e] = 0.f;
-                g[e] = g1;
             }
-            if (a.dx) rn_store<VEC>(a.dx, a.x_bf, row * d + c, t);
-            if (a.post_w) rn_load<VEC>(a.post_w, 0, c, w);
-            if (a.post_b) rn_load<VEC>(a.post_b, 0, c, b);
-            if (a.gate_mode == 2) rn_load<VEC>(a.gate, 0, grp * d + c, g);
-            if (a.scale) rn_load<VEC>(a.scale, 0, c, sc);
+            if (a.dx) rn_store(a.dx, TX == 2 ? a.x_bf : TX, row * d, c, d, t);
+            const float4 w4 = vec(1, i), b4 = vec(2, i), s4 = vec(3, i);
+            const float w[4] = {w4.x, w4.y, w4.z, w4.w}, b[4] = {b4.x, b4.y, b4.z, b4.w}, sc[4] = {s4.x, s4.y, s4.z, s4.w};
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
+            for (int e = 0; e < 4; ++e) {
+                const float g = GC ? gate[GC ? i : 0][e] : cur.g;
                 const float hat = (hv[i][e] - mean) * rstd;          // post_w null: h itself
-                const float p = fmaf(hat, w[e], b[e]), pg = p * gy[i][e];
-                const float m = g[e] * sc[e];
-                dp[e] = m == 0.f ? 0.f : m * gy[i][e];
-                cs[2][i][e] = g[e] == 0.f ? cs[2][i][e] : fmaf(g[e], pg, cs[2][i][e]);
-                cg[i][e] = fmaf(sc[e], pg, cg[i][e]);
-                s[2] = fmaf(sc[e], pg, s[2]);
-                cs[0][i][e] = dp[e] == 0.f ? cs[0][i][e] : fmaf(dp[e], hat, cs[0][i][e]);
-                cs[1][i][e] += dp[e];
-                const float v = dp[e] * w[e];
+                const float m = g * sc[e];
+                const float dp = m == 0.f ? 0.f : m * gy[i][e];
+                if constexpr (GC) {
+                    cg[0][i][e] = fmaf(gy[i][e], hat, cg[0][i][e]);
+                    cg[GC][i][e] += gy[i][e];
+                } else {
+                    const float q = g * gy[i][e];
+                    cs[0][i][e] = g == 0.f ? cs[0][i][e] : fmaf(q, hat, cs[0][i][e]);
+                    cs[1][i][e] += q;
+                    s[2] = c + e < d ? fmaf(sc[e] * gy[i][e], fmaf(hat, w[e], b[e]), s[2]) : s[2];
+                }
+                const float v = dp * w[e];
                 s[0] += v;
                 s[1] = v == 0.f ? s[1] : fmaf(v, hat, s[1]);
                 gy[i][e] = v;
                 hv[i][e] = hat;
             }
         }
-        if (a.post_w || a.gate_mode == 1) team_sum<W>(s, sh);
-        if (a.gate_mode == 1 && lane == 0) (a.groups == a.rows ? a.dgate : a.gate_rows)[row] = s[2];
+        if (a.post_w || (!GC && a.gate_mode == 1)) team_sum<W>(s, red);
+        if (!GC && a.gate_mode == 1 && lane == 0) (a.groups == a.rows ? a.dgate : a.gate_rows)[row] = s[2];
         if (a.dh) {
             const float m1 = a.rms ? 0.f : s[0] * a.inv_d, m2 = s[1] * a.inv_d;
 #pragma unroll
@@ -346,33 +474,42 @@ __global__ __launch_bounds__(64 * W * TEAMS) void residual_norm_bwd_kernel(RnArg
                 if (c >= d) continue;
                 if (a.post_w) {
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
+                    for (int e = 0; e < 4; ++e) {
                         const float v = gy[i][e] - m1 - (m2 == 0.f ? 0.f : hv[i][e] * m2);
                         gy[i][e] = v == 0.f ? 0.f : rstd * v;
                     }
                 }
-                rn_store<VEC>(a.dh, a.h_bf, row * d + c, gy[i]);
+                rn_store(a.dh, THZ == 2 ? a.h_bf : THZ, row * d, c, d, gy[i]);
             }
         }
-        if (a.gate_mode) {
-            // a group's rows are neighbours: its gate's row of column sums is handed over where the group (or this team's part of
-            // it) ends.  Slot team + group: both only grow along the rows, so no two (team, group) pairs share one.
+        if constexpr (GC) {
+            // a group's rows are neighbours: its sums are handed over where the group (or this team's part of it) ends, its gate's row of
+            // gradients into slot team + group: both only grow along the rows, so no two (team, group) pairs share one
             const bool last = ++in_grp == a.rpg;
-            if (a.gate_mode == 2 && (last || row + 1 == r1)) {
+            if (last || row + 1 == r1) {
                 float* out = a.groups == a.rows ? a.dgate + grp * d : a.gate_rows + (team + grp) * d;
 #pragma unroll
                 for (int i = 0; i < NCH; ++i) {
                     const int c = c0 + i * STEP;
-                    if (c < d) rn_store<VEC>(out, 0, c, cg[i]);
+                    if (c >= d) continue;
+                    const float4 w4 = vec(1, i), b4 = vec(2, i), s4 = vec(3, i);
+                    const float w[4] = {w4.x, w4.y, w4.z, w4.w}, b[4] = {b4.x, b4.y, b4.z, b4.w}, sc[4] = {s4.x, s4.y, s4.z, s4.w};
+                    float t[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float g = gate[i][e], A = cg[0][i][e], B = cg[GC][i][e];
+                        t[e] = sc[e] * fmaf(w[e], A, b[e] * B);
+                        cs[0][i][e] = g == 0.f ? cs[0][i][e] : fmaf(g, A, cs[0][i][e]);
+                        cs[1][i][e] = fmaf(g, B, cs[1][i][e]);
+                        cg[0][i][e] = cg[GC][i][e] = 0.f;
+                    }
+                    rn_store(out, 0, 0, c, d, t);
                 }
-#pragma unroll
-                for (int i = 0; i < NCH; ++i)
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) cg[i][e] = 0.f;
             }
             if (last) {
                 ++grp;
                 in_grp = 0;
+                if (row + 1 < r1) load_gate();
             }
         }
     }
@@ -383,10 +520,9 @@ __global__ __launch_bounds__(64 * W * TEAMS) void residual_norm_bwd_kernel(RnArg
             __syncthreads();
 #pragma unroll
             for (int i = 0; i < NCH; ++i)
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) sh[team_in * COLS + c0 + i * STEP + e] = cs[k][i][e];
+                *reinterpret_cast<float4*>(sh + team_in * COLS + c0 + i * STEP) = make_float4(cs[k][i][0], cs[k][i][1], cs[k][i][2], cs[k][i][3]);
             __syncthreads();
-            for (int c = threadIdx.x; c < d; c += 64 * TEAMS) {
+            for (int c = threadIdx.x; c < d; c += NT) {
                 float t = 0.f;
 #pragma unroll
                 for (int w = 0; w < TEAMS; ++w) t += sh[w * COLS + c];
@@ -399,81 +535,99 @@ __global__ __launch_bounds__(64 * W * TEAMS) void residual_norm_bwd_kernel(RnArg
 #pragma unroll
             for (int i = 0; i < NCH; ++i) {
                 const int c = c0 + i * STEP;
-                if (c < d) rn_store<VEC>(out + k * d, 0, c, cs[k][i]);
+                if (c < d) rn_store(out, 0, k * (int64_t)d, c, d, cs[k][i]);
             }
     }
 }
 
 struct RnFinish {
-    const float* part;
-    const float* gate_rows;
-    float* out[RN_KINDS];
-    float* dgate;
+    const float *part, *gate_rows, *post_w, *post_b, *scale;
+    float *dpost_w, *dpost_b, *dscale, *dpre_w, *dpre_b, *dgate;
     int nblk, d, col_blocks, gate_mode, rows_per_team;
-    int64_t groups, rpg, rows;
+    int64_t groups, rpg;
 };
 
-// workgroups 0 .. 5 col_blocks - 1: 64 columns of one column sum, four threads to a column over a quarter of the blocks each;
-// behind them the gate: 4 groups to a workgroup (a number per group) or 64 columns of one group (a row per group)
+// workgroups 0 .. 3 col_blocks - 1: 16 columns of the sums that belong together (those of the norm before, d weight and d bias of the one
+// after), 16 threads to a column over a sixteenth of the blocks each, eight loads of a thread under way at a time (four threads to a
+// column took 19 us, as long as a quarter of the rows' pass); behind them the gate: 4 groups to a workgroup (a number per group) or 256
+// columns of one group (a row per group)
 __global__ __launch_bounds__(256) void residual_norm_finish_kernel(RnFinish f) {
-    __shared__ float sh[4][64];
-    const int col = threadIdx.x & 63, q = threadIdx.x >> 6;
+    __shared__ float sh[2][16][17];
     int64_t b = blockIdx.x;
-    if (b < RN_KINDS * f.col_blocks) {
-        const int k = (int)b / f.col_blocks, c = ((int)b % f.col_blocks) * 64 + col;
-        if (!f.out[k]) return;
-        float s = 0.f;
-        if (c < f.d)
-            for (int i = q; i < f.nblk; i += 4) s += f.part[((int64_t)i * RN_KINDS + k) * f.d + c];
-        sh[q][col] = s;
+    if (b < 3 * f.col_blocks) {
+        const int col = threadIdx.x & 15, q = threadIdx.x >> 4;
+        const int k = (int)b / f.col_blocks, c = ((int)b % f.col_blocks) * 16 + col;
+        if (k == 0 ? !(f.dpost_w || f.dpost_b || f.dscale) : k == 1 ? !f.dpre_w : !f.dpre_b) return;
+        const float* p = f.part + (int64_t)(k == 0 ? 0 : k + 1) * f.d + (c < f.d ? c : 0);
+        const int64_t step = (int64_t)RN_KINDS * f.d;
+        float s = 0.f, t = 0.f;
+        if (k == 0) {
+#pragma unroll 8
+            for (int i = q; i < f.nblk; i += 16) {
+                s += p[i * step];
+                t += p[i * step + f.d];
+            }
+        } else {
+#pragma unroll 8
+            for (int i = q; i < f.nblk; i += 16) s += p[i * step];
+        }
+        sh[0][q][col] = s;
+        sh[1][q][col] = t;
         __syncthreads();
-        if (q == 0 && c < f.d) f.out[k][c] = (sh[0][col] + sh[1][col]) + (sh[2][col] + sh[3][col]);
+        if (q || c >= f.d) return;
+        float A = 0.f, B = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            A += sh[0][i][col];
+            B += sh[1][i][col];
+        }
+        if (k == 1) f.dpre_w[c] = A;
+        else if (k == 2) f.dpre_b[c] = A;
+        else {
+            const float sc = f.scale ? f.scale[c] : 1.f;
+            if (f.dpost_w) f.dpost_w[c] = sc == 0.f ? 0.f : sc * A;
+            if (f.dpost_b) f.dpost_b[c] = sc == 0.f ? 0.f : sc * B;
+            if (f.dscale) f.dscale[c] = fmaf(f.post_w ? f.post_w[c] : 1.f, A, f.post_b ? f.post_b[c] * B : 0.f);
+        }
         return;
     }
-    b -= RN_KINDS * f.col_blocks;
+    b -= 3 * f.col_blocks;
+    const int col = threadIdx.x & 63, q = threadIdx.x >> 6;
     if (f.gate_mode == 1) {
         const int64_t g = b * 4 + q;
         if (g >= f.groups) return;
         float s = 0.f;
         for (int64_t r = col; r < f.rpg; r += 64) s += f.gate_rows[g * f.rpg + r];
-        s = wave_sum(s);
+        s = row_add_sum(s);
         if (col == 0) f.dgate[g] = s;
     } else {
-        const int64_t g = b / f.col_blocks;
-        const int c = (int)(b % f.col_blocks) * 64 + col;
+        const int blocks = (f.d + 255) / 256;
+        const int64_t g = b / blocks;
+        const int c = (int)(b % blocks) * 256 + threadIdx.x;
+        if (c >= f.d) return;
         const int64_t t0 = g * f.rpg / f.rows_per_team, t1 = ((g + 1) * f.rpg - 1) / f.rows_per_team;
         float s = 0.f;
-        if (c < f.d)
-            for (int64_t t = t0 + q; t <= t1; t += 4) s += f.gate_rows[(t + g) * f.d + c];
-        sh[q][col] = s;
-        __syncthreads();
-        if (q == 0 && c < f.d) f.dgate[g * f.d + c] = (sh[0][col] + sh[1][col]) + (sh[2][col] + sh[3][col]);
+#pragma unroll 8
+        for (int64_t t = t0; t <= t1; ++t) s += f.gate_rows[(t + g) * f.d + c];
+        f.dgate[g * f.d + c] = s;
     }
 }
 
-static bool aligned(const void* p, int bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
-
 struct RnPlan {
-    int W, nch, vec, teams, rows_per_team, blocks;
+    int W, nch, teams, rows_per_team, blocks;
 };
 
-// One wave to a row up to 1 024 columns (16 values of a tensor to a lane), whole workgroups beyond: no barrier inside a row where
-// one wave holds it.  Backward: at least RN_MIN_ROWS rows to a team, so the teams' column sums stay small beside the rows, and at
-// most one workgroup of eight waves to each of the 256 CUs.
-constexpr int RN_MIN_ROWS = 4;
-static RnPlan rn_plan(int rows, int d, bool vec4) {
+// Forward: one wave to a row up to 1 024 columns (no barrier inside a row), four up to 4 096, eight beyond.  Backward: a wave to a row up to 768
+// columns, four up to 2 048, eight beyond, because it keeps more of a row and the column sums in registers (16448 x 1024 with a row of
+// gates: 75 us, 163 with one wave to a row and spilled registers); at most one workgroup of eight waves to each of the 256 CUs (two of
+// four, four where a lane has one vector): every workgroup leaves four rows of column sums, 2 to 8 % of what the rows are.
+static RnPlan rn_plan(int rows, int d, bool bwd) {
     RnPlan p;
-    p.vec = vec4 ? 4 : 1;
-    p.W = d <= 1024 ? 1 : d <= 4096 ? 4 : 8;
-    const int per = 64 * p.W * p.vec, need = (d + per - 1) / per;
-    p.nch = 1;
-    if (vec4 && p.W == 1) p.nch = need;
-    else
-        while (p.nch < need) p.nch *= 2;
-    if (!vec4 && p.nch < 4) p.nch = 4;
-    const int teams_blk = p.W == 1 ? 8 : 1, most = 256 * (p.W == 1 ? 8 : p.W == 4 ? 2 : 1);
-    int teams = (rows + RN_MIN_ROWS - 1) / RN_MIN_ROWS;
-    if (teams > most) teams = most;
+    p.W = d <= (bwd ? 768 : 1024) ? 1 : d <= (bwd ? 2048 : 4096) ? 4 : 8;
+    const int need = (d + 256 * p.W - 1) / (256 * p.W);
+    p.nch = need == 3 && p.W > 1 ? 4 : need;
+    const int teams_blk = p.W == 1 ? 8 : 1, most = 256 * (p.W == 1 ? 8 : p.W == 4 ? (p.nch == 1 ? 4 : 2) : 1);
+    const int teams = rows < most ? rows : most;
     p.rows_per_team = rows ? (rows + teams - 1) / teams : 1;
     p.teams = rows ? (rows + p.rows_per_team - 1) / p.rows_per_team : 0;
     p.blocks = (p.teams + teams_blk - 1) / teams_blk;
@@ -481,16 +635,10 @@ static RnPlan rn_plan(int rows, int d, bool vec4) {
     return p;
 }
 
-#define RN_CASE(W_, N_, V_) \
-    if (p.W == W_ && p.nch == N_ && p.vec == V_) return launch(std::integral_constant<int, W_>{}, std::integral_constant<int, N_>{}, std::integral_constant<int, V_>{});
-
-template <typename F>
-static bool rn_dispatch(const RnPlan& p, F&& launch) {
-    RN_CASE(1, 1, 4) RN_CASE(1, 2, 4) RN_CASE(1, 3, 4) RN_CASE(1, 4, 4) RN_CASE(4, 2, 4) RN_CASE(4, 4, 4) RN_CASE(8, 4, 4)
-    RN_CASE(1, 4, 1) RN_CASE(1, 8, 1) RN_CASE(1, 16, 1) RN_CASE(4, 8, 1) RN_CASE(4, 16, 1) RN_CASE(8, 16, 1)
-    return false;
+template <int W, int... N, typename F>
+static bool rn_try(const RnPlan& p, F&& launch) {   // W and one of N vectors to a lane
+    return p.W == W && ((p.nch == N && (launch(std::integral_constant<int, W>{}, std::integral_constant<int, N>{}), true)) || ...);
 }
-#undef RN_CASE
 
 static int rn_common(RnArgs& a, int rows, int d, int64_t groups, int gate_channels, const char* what) {
     SWAT_REQUIRE(rows >= 0 && d >= 1 && d <= 8192, "%s: rows %d, width %d (0 rows or more, 1 to 8192 columns)", what, rows, d);
@@ -505,8 +653,6 @@ static int rn_common(RnArgs& a, int rows, int d, int64_t groups, int gate_channe
     a.gate_mode = a.gate ? (gate_channels ? 2 : 1) : 0;
     return 0;
 }
-
-static bool vec_ok(const void* p, int bf, int64_t stride) { return !p || (aligned(p, bf ? 8 : 16) && stride % 4 == 0); }
 
 }  // namespace swat
 
@@ -529,23 +675,18 @@ SWAT_API int swat_residual_norm_fwd(const void* x, int64_t x_stride, int x_dtype
     a.y = y; a.z = z; a.z8 = (unsigned char*)z8_codes; a.z8s = (unsigned char*)z8_scales; a.stats = stats;
     a.z8s_ld = (d + 31) / 32;
     a.z8_ld = 32 * a.z8s_ld;
-    const bool v = d % 4 == 0 && vec_ok(x, a.x_bf, x_stride) && vec_ok(h, a.h_bf, h_stride) && vec_ok(y, a.x_bf, d) && vec_ok(z, a.z_bf, d) &&
-                   vec_ok(post_w, 0, 0) && vec_ok(post_b, 0, 0) && vec_ok(gate_channels ? gate : nullptr, 0, 0) && vec_ok(scale, 0, 0) &&
-                   vec_ok(pre_w, 0, 0) && vec_ok(pre_b, 0, 0) && aligned(z8_codes, 4);
-    const RnPlan p = rn_plan(rows, d, v);
-    const hipStream_t s = (hipStream_t)stream;
-    const bool known = rn_dispatch(p, [&](auto w, auto n, auto c) {
-        constexpr int W = decltype(w)::value, N = decltype(n)::value, V = decltype(c)::value;
-        const int grid = W == 1 ? (rows + 3) / 4 : rows;
-        residual_norm_fwd_kernel<W, N, V><<<grid, W == 1 ? 256 : 64 * W, 0, s>>>(a);
-        return true;
-    });
-    SWAT_REQUIRE(known, "swat_residual_norm_fwd: no kernel for %d columns", d);
+    SWAT_REQUIRE(((uintptr_t)z8_codes & 3) == 0, "swat_residual_norm_fwd: codes sit on 4 bytes");
+    const RnPlan p = rn_plan(rows, d, false);
+    auto go = [&](auto w, auto n) {
+        constexpr int W = decltype(w)::value, N = decltype(n)::value;
+        residual_norm_fwd_kernel<W, N><<<W == 1 ? (rows + 3) / 4 : rows, W == 1 ? 256 : 64 * W, 0, (hipStream_t)stream>>>(a);
+    };
+    SWAT_REQUIRE((rn_try<1, 1, 2, 3, 4>(p, go) || rn_try<4, 2, 4>(p, go) || rn_try<8, 4>(p, go)), "swat_residual_norm_fwd: no kernel for %d columns", d);
     return check_launch("swat_residual_norm_fwd");
 }
 
-static int64_t rn_ws(int rows, int d, int64_t groups, int gate_mode, bool vec4, int64_t* gate_at) {
-    const RnPlan p = rn_plan(rows, d, vec4);
+static int64_t rn_ws(int rows, int d, int64_t groups, int gate_mode, int64_t* gate_at) {
+    const RnPlan p = rn_plan(rows, d, true);
     *gate_at = (int64_t)p.blocks * RN_KINDS * d;
     const int64_t slots = gate_mode == 1 ? rows : gate_mode == 2 ? (p.teams + groups) * (int64_t)d : 0;
     return 4 * (*gate_at + slots);
@@ -556,10 +697,8 @@ SWAT_API int64_t swat_residual_norm_bwd_workspace_bytes(int rows, int d, int64_t
         set_error("swat_residual_norm_bwd_workspace_bytes: rows %d, width %d, groups %lld", rows, d, (long long)groups);
         return -1;
     }
-    int64_t at;  // (alignment decides the vector width at the call: room for either plan)
-    const int mode = groups ? (gate_channels ? 2 : 1) : 0;
-    const int64_t n = rn_ws(rows, d, groups, mode, true, &at), m = rn_ws(rows, d, groups, mode, false, &at);
-    return n > m ? n : m;
+    int64_t at;
+    return rn_ws(rows, d, groups, groups ? (gate_channels ? 2 : 1) : 0, &at);
 }
 
 SWAT_API int swat_residual_norm_bwd(const void* dy, int64_t dy_stride, const void* dz, int64_t dz_stride, int z_dtype, const void* h,
@@ -582,35 +721,43 @@ SWAT_API int swat_residual_norm_bwd(const void* dy, int64_t dy_stride, const voi
     a.x_bf = x_dtype == SWAT_BF16; a.h_bf = h_dtype == SWAT_BF16; a.z_bf = z_dtype == SWAT_BF16;
     a.alpha = alpha; a.rms = rms != 0; a.stats = const_cast<float*>(stats);
     a.dx = dx; a.dh = dh; a.dgate = dgate;
-    const bool v = d % 4 == 0 && vec_ok(dy, a.x_bf, dy_stride) && vec_ok(dz, a.z_bf, dz_stride) && vec_ok(h, a.h_bf, h_stride) &&
-                   vec_ok(y, a.x_bf, y_stride) && vec_ok(dx, a.x_bf, d) && vec_ok(dh, a.h_bf, d) && vec_ok(post_w, 0, 0) &&
-                   vec_ok(post_b, 0, 0) && vec_ok(gate_channels ? gate : nullptr, 0, 0) && vec_ok(scale, 0, 0) && vec_ok(pre_w, 0, 0) &&
-                   vec_ok(gate_channels ? dgate : nullptr, 0, 0) && aligned(workspace, 16);
-    const RnPlan p = rn_plan(rows, d, v);
+    const RnPlan p = rn_plan(rows, d, true);
     int64_t gate_at;
-    const int64_t want = rn_ws(rows, d, a.groups, a.gate_mode, v, &gate_at);
-    SWAT_REQUIRE(rows == 0 || (workspace && workspace_bytes >= want), "swat_residual_norm_bwd: workspace of %lld bytes, %lld are needed", (long long)workspace_bytes, (long long)want);
+    const int64_t want = rn_ws(rows, d, a.groups, a.gate_mode, &gate_at);
+    SWAT_REQUIRE(rows == 0 || (workspace && workspace_bytes >= want && ((uintptr_t)workspace & 15) == 0),
+                 "swat_residual_norm_bwd: workspace of %lld bytes, %lld on 16 bytes are needed", (long long)workspace_bytes, (long long)want);
     a.part = (float*)workspace;
     a.gate_rows = a.part + gate_at;
     a.rows_per_team = p.rows_per_team;
     const hipStream_t s = (hipStream_t)stream;
     if (rows > 0) {
-        const bool known = rn_dispatch(p, [&](auto w, auto n, auto c) {
-            constexpr int W = decltype(w)::value, N = decltype(n)::value, V = decltype(c)::value, T = W == 1 ? 8 : 1;
-            residual_norm_bwd_kernel<W, N, V, T><<<p.blocks, 64 * W * T, 0, s>>>(a);
-            return true;
-        });
-        SWAT_REQUIRE(known, "swat_residual_norm_bwd: no kernel for %d columns", d);
+        auto run = [&](auto w, auto n) {
+            constexpr int W = decltype(w)::value, N = decltype(n)::value, T = W == 1 ? 8 : 1;
+            const bool hz_bf = a.h_bf && (a.z_bf || !dz), gc = a.gate_mode == 2;
+            auto go = [&](auto tx, auto thz) {
+                constexpr int TX = decltype(tx)::value, THZ = decltype(thz)::value;
+                if (gc) residual_norm_bwd_kernel<W, N, T, TX, THZ, true><<<p.blocks, 64 * W * T, 0, s>>>(a);
+                else residual_norm_bwd_kernel<W, N, T, TX, THZ, false><<<p.blocks, 64 * W * T, 0, s>>>(a);
+            };
+            using I0 = std::integral_constant<int, 0>;
+            using I1 = std::integral_constant<int, 1>;
+            using I2 = std::integral_constant<int, 2>;
+            if (hz_bf && !a.x_bf) go(I0{}, I1{});
+            else if (hz_bf) go(I1{}, I1{});
+            else go(I2{}, I2{});
+        };
+        SWAT_REQUIRE((rn_try<1, 1, 2, 3>(p, run) || rn_try<4, 1, 2>(p, run) || rn_try<8, 2, 4>(p, run)), "swat_residual_norm_bwd: no kernel for %d columns", d);
     }
     RnFinish f = {};
-    f.part = a.part; f.gate_rows = a.gate_rows; f.nblk = p.blocks; f.d = d; f.col_blocks = (d + 63) / 64;
-    f.out[0] = post_w ? dpost_w : nullptr; f.out[1] = post_b ? dpost_b : nullptr; f.out[2] = scale ? dscale : nullptr;
-    f.out[3] = pre_w ? dpre_w : nullptr; f.out[4] = pre_b ? dpre_b : nullptr;
-    f.dgate = dgate; f.groups = a.groups; f.rpg = a.rpg; f.rows = rows; f.rows_per_team = p.rows_per_team;
+    f.part = a.part; f.gate_rows = a.gate_rows; f.nblk = p.blocks; f.d = d; f.col_blocks = (d + 15) / 16;
+    f.post_w = post_w; f.post_b = post_b; f.scale = scale;
+    f.dpost_w = post_w ? dpost_w : nullptr; f.dpost_b = post_b ? dpost_b : nullptr; f.dscale = scale ? dscale : nullptr;
+    f.dpre_w = pre_w ? dpre_w : nullptr; f.dpre_b = pre_b ? dpre_b : nullptr;
+    f.dgate = dgate; f.groups = a.groups; f.rpg = a.rpg; f.rows_per_team = p.rows_per_team;
     f.gate_mode = a.groups != rows ? a.gate_mode : 0;
     if (rows == 0) f.rpg = 0;  // sums over nothing: zeros
-    int64_t grid = RN_KINDS * f.col_blocks;
-    grid += f.gate_mode == 1 ? (f.groups + 3) / 4 : f.gate_mode == 2 ? f.groups * f.col_blocks : 0;
+    int64_t grid = 3 * f.col_blocks;
+    grid += f.gate_mode == 1 ? (f.groups + 3) / 4 : f.gate_mode == 2 ? f.groups * ((d + 255) / 256) : 0;
     residual_norm_finish_kernel<<<(unsigned)grid, 256, 0, s>>>(f);
     return check_launch("swat_residual_norm_bwd");
 }

@@ -10,7 +10,6 @@ from collections import namedtuple
 import torch
 
 from . import _lib
-from ._lib import ptr as _p
 from .ops import ACT
 
 _BF, _F32 = torch.bfloat16, torch.float32
@@ -30,23 +29,24 @@ class MX(namedtuple("MX", "codes scale cols bits")):
         return (self.codes.shape[0], self.cols)
 
 
-def _empty(rows, cols, bits, dev):
+def _empty(like, rows, cols, bits):
     blocks = (cols + 31) // 32
-    return MX(torch.empty((rows, blocks * 4 * bits), dtype=torch.uint8, device=dev), torch.empty((rows, blocks), dtype=torch.uint8, device=dev),
-              cols, bits)
+    return MX(like.new_empty((rows, blocks * 4 * bits), dtype=torch.uint8), like.new_empty((rows, blocks), dtype=torch.uint8), cols, bits)
 
 
 def _check(m, what, bits=(4, 8)):
+    """The pointers of an MX matrix whose parts fit together, on the current device."""
     if not isinstance(m, MX) or m.bits not in bits or m.cols < 1:
         raise _lib.SwatHipError(f"{what}: an MX matrix of {' or '.join(map(str, bits))} bits is wanted, got {m!r:.80}")
-    rows, blocks = m.codes.shape[0], (m.cols + 31) // 32
-    if (m.codes.dtype != torch.uint8 or m.scale.dtype != torch.uint8 or m.codes.shape != (rows, blocks * 4 * m.bits)
-            or m.scale.shape != (rows, blocks)):
-        raise _lib.SwatHipError(f"{what}: codes {tuple(m.codes.shape)} {m.codes.dtype} and scale {tuple(m.scale.shape)} {m.scale.dtype} are not "
-                                f"those of {m.cols} columns in {m.bits} bits")
-    _lib.on_device(m.codes, what)
-    _lib.on_device(m.scale, what)
-    return _p(m.codes), _p(m.scale)
+    codes, scale = m.codes, m.scale
+    rows, blocks = codes.shape[0], (m.cols + 31) // 32
+    if (codes.dtype != torch.uint8 or scale.dtype != torch.uint8 or codes.shape != (rows, blocks * 4 * m.bits) or scale.shape != (rows, blocks)
+            or not codes.is_cuda or not scale.is_cuda or codes.get_device() != _lib._current() or scale.get_device() != _lib._current()
+            or not codes.is_contiguous() or not scale.is_contiguous()):
+        raise _lib.SwatHipError(f"{what}: codes {tuple(codes.shape)} {codes.dtype} on {codes.device}, scale {tuple(scale.shape)} {scale.dtype} on "
+                                f"{scale.device} are not the contiguous parts of {m.cols} columns in {m.bits} bits on the current device "
+                                "(no CPU fallback)")
+    return codes.data_ptr(), scale.data_ptr()
 
 
 def _act(act, what):
@@ -60,9 +60,9 @@ def quantize(x, bits=8):
     px, ld = _lib.rows_ptr(x, "mx.quantize", (_BF, _F32))
     if bits not in (4, 8) or x.shape[1] < 1:
         raise _lib.SwatHipError(f"mx.quantize: {bits} bits (4 or 8) of {x.shape[1]} columns (1 at least)")
-    m = _empty(x.shape[0], x.shape[1], bits, x.device)
-    _lib.check(_lib.lib().swat_mx_quantize(px, ld, int(x.dtype == _BF), bits, _p(m.codes), _p(m.scale), x.shape[0], x.shape[1], _lib.stream()),
-               "swat_mx_quantize")
+    m = _empty(x, x.shape[0], x.shape[1], bits)
+    _lib.check(_lib.lib().swat_mx_quantize(px, ld, x.dtype == _BF, bits, m.codes.data_ptr(), m.scale.data_ptr(), x.shape[0], x.shape[1],
+                                           _lib.stream()), "swat_mx_quantize")
     return m
 
 
@@ -71,8 +71,8 @@ def dequantize(m, dtype=_BF):
     codes, scale = _check(m, "mx.dequantize")
     if dtype not in (_BF, _F32):
         raise _lib.SwatHipError(f"mx.dequantize: {dtype} (bfloat16 or float32)")
-    out = torch.empty(m.shape, dtype=dtype, device=m.codes.device)
-    _lib.check(_lib.lib().swat_mx_dequantize(codes, scale, m.bits, _p(out), int(dtype == _BF), m.rows, m.cols, _lib.stream()),
+    out = m.codes.new_empty(m.shape, dtype=dtype)
+    _lib.check(_lib.lib().swat_mx_dequantize(codes, scale, m.bits, out.data_ptr(), dtype == _BF, m.rows, m.cols, _lib.stream()),
                "swat_mx_dequantize")
     return out
 
@@ -83,9 +83,10 @@ def act_fwd(f, act="gelu"):
     a = _act(act, "mx.act_fwd")
     if f.shape[1] < 1:
         raise _lib.SwatHipError("mx.act_fwd: no columns")
-    m = _empty(f.shape[0], f.shape[1], 8, f.device)
-    g = torch.empty(f.shape, dtype=_BF, device=f.device)
-    _lib.check(_lib.lib().swat_mx_act_fwd(pf, ld, a, _p(g), _p(m.codes), _p(m.scale), f.shape[0], f.shape[1], _lib.stream()), "swat_mx_act_fwd")
+    m = _empty(f, f.shape[0], f.shape[1], 8)
+    g = f.new_empty(f.shape)
+    _lib.check(_lib.lib().swat_mx_act_fwd(pf, ld, a, g.data_ptr(), m.codes.data_ptr(), m.scale.data_ptr(), f.shape[0], f.shape[1],
+                                          _lib.stream()), "swat_mx_act_fwd")
     return g, m
 
 
@@ -96,9 +97,10 @@ def act_bwd(dg, m, act="gelu", want_act=True):
     a = _act(act, "mx.act_bwd")
     if dg.shape[0] != m.rows:
         raise _lib.SwatHipError(f"mx.act_bwd: {dg.shape[0]} rows of dg, {m.rows} of the checkpoint")
-    df = torch.empty(m.shape, dtype=_BF, device=dg.device)
-    g = torch.empty(m.shape, dtype=_BF, device=dg.device) if want_act else None
-    _lib.check(_lib.lib().swat_mx_act_bwd(pg, ld, codes, scale, a, _p(df), _p(g), m.rows, m.cols, _lib.stream()), "swat_mx_act_bwd")
+    df = dg.new_empty(m.shape)
+    g = dg.new_empty(m.shape) if want_act else None
+    _lib.check(_lib.lib().swat_mx_act_bwd(pg, ld, codes, scale, a, df.data_ptr(), g.data_ptr() if want_act else None, m.rows, m.cols,
+                                          _lib.stream()), "swat_mx_act_bwd")
     return df, g
 
 
@@ -110,13 +112,14 @@ def linear_wgrad(dy, m, want_bias=False, out=None):
     if rows != m.rows:
         raise _lib.SwatHipError(f"mx.linear_wgrad: {rows} rows of dy, {m.rows} of the checkpoint")
     if out is None:
-        out = torch.empty((n, m.cols), dtype=_F32, device=dy.device)
-    pw = _lib.vec_ptr(out, "mx.linear_wgrad: out", (n, m.cols))
-    db = torch.empty(n, dtype=_F32, device=dy.device) if want_bias else None
+        out = dy.new_empty((n, m.cols), dtype=_F32)
+    pw = _lib.vec_ptr(out, "mx.linear_wgrad: out", n, m.cols)
+    db = dy.new_empty(n, dtype=_F32) if want_bias else None
     h = _lib.lib()
     nbytes = h.swat_mx_linear_wgrad_workspace_bytes(rows, n, m.cols)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dy.device) if nbytes > 0 else None
-    _lib.check(h.swat_mx_linear_wgrad(py, ld, codes, scale, pw, _p(db), rows, n, m.cols, _p(ws), nbytes, _lib.stream()), "swat_mx_linear_wgrad")
+    ws = dy.new_empty(nbytes, dtype=torch.uint8) if nbytes > 0 else None
+    _lib.check(h.swat_mx_linear_wgrad(py, ld, codes, scale, pw, db.data_ptr() if want_bias else None, rows, n, m.cols,
+                                      ws.data_ptr() if nbytes > 0 else None, nbytes, _lib.stream()), "swat_mx_linear_wgrad")
     return (out, db) if want_bias else out
 
 
@@ -128,8 +131,8 @@ def matmul(a, b, bias=None, out_dtype=_BF):
     if a.cols != b.cols or not (out_dtype == _BF or (out_dtype == _F32 and a.bits == b.bits == 4)):
         raise _lib.SwatHipError(f"mx.matmul: {a.shape} in {a.bits} bits by {b.shape} in {b.bits} bits (the same columns) into {out_dtype} "
                                 "(bfloat16; float32 where both have 4 bits)")
-    pb = _lib.vec_ptr(bias, "mx.matmul: bias", (b.rows,))
-    c = torch.empty((a.rows, b.rows), dtype=out_dtype, device=a.codes.device)
-    _lib.check(_lib.lib().swat_mx_matmul(ca, sa, a.bits, cb, sb, b.bits, pb, _p(c), int(out_dtype == _BF), a.rows, b.rows, a.cols, _lib.stream()),
+    pb = _lib.vec_ptr(bias, "mx.matmul: bias", b.codes.shape[0])
+    c = a.codes.new_empty((a.rows, b.rows), dtype=out_dtype)
+    _lib.check(_lib.lib().swat_mx_matmul(ca, sa, a.bits, cb, sb, b.bits, pb, c.data_ptr(), out_dtype == _BF, a.rows, b.rows, a.cols, _lib.stream()),
                "swat_mx_matmul")
     return c

@@ -105,20 +105,21 @@ ResidualNorm = namedtuple("ResidualNorm", "y z stats z8")
 
 def _seam(what, rows, d, post, pre, gate, scale, norm):
     """The checked pointers of what both directions of the seam take: post w, b, gate, groups, per channel, scale, pre w, b, rms."""
-    if norm not in ("layer", "rms"):
+    if norm != "layer" and norm != "rms":
         raise _lib.SwatHipError(f"{what}: norm {norm!r} ('layer' or 'rms')")
-    v, groups, channels = [], 0, 0
-    for name, wb in (("post", post), ("pre", pre)):
-        w, b = wb if wb is not None else (None, None)
-        if wb is not None and w is None:
-            raise _lib.SwatHipError(f"{what}: {name} = (weight, bias or None)")
-        v += [_lib.vec_ptr(w, f"{what}: {name} weight", (d,)), _lib.vec_ptr(b, f"{what}: {name} bias", (d,))]
+    pw, pb = post if post is not None else (None, None)
+    qw, qb = pre if pre is not None else (None, None)
+    if (post is not None and pw is None) or (pre is not None and qw is None):
+        raise _lib.SwatHipError(f"{what}: post, pre = (weight, bias or None)")
+    vec = _lib.vec_ptr
+    g, groups, channels = None, 0, 0
     if gate is not None:
         groups, channels = gate.shape[0], int(gate.dim() == 2)
-        g = _lib.vec_ptr(gate, f"{what}: gate", (groups, d) if channels else (groups,))
+        g = vec(gate, what, groups, d) if channels else vec(gate, what, groups)
         if groups < 1 or rows % groups:
             raise _lib.SwatHipError(f"{what}: {groups} gates do not divide {rows} rows")
-    return v[0], v[1], g if gate is not None else None, groups, channels, _lib.vec_ptr(scale, f"{what}: scale", (d,)), v[2], v[3], int(norm == "rms")
+    return (vec(pw, what, d), vec(pb, what, d), g, groups, channels, vec(scale, what, d), vec(qw, what, d), vec(qb, what, d),
+            int(norm == "rms"))
 
 
 def residual_norm_fwd(x, h, post=None, pre=None, gate=None, scale=None, alpha=1.0, norm="layer", eps=1e-5, z_dtype=_BF, pack=False):
@@ -129,25 +130,23 @@ def residual_norm_fwd(x, h, post=None, pre=None, gate=None, scale=None, alpha=1.
     [groups] or [groups, d], for rows / groups neighbouring rows each (stochastic depth: 0 or 1 / keep per image).  Where gate * scale is
     zero nothing of h is taken.  y has x's type, z z_dtype; stats fp32 [4, rows] is for residual_norm_bwd; pack: z8 = z as an 8-bit
     microscaled matrix (mx.MX), the checkpoint of the next linear layer's input or an operand of mx.matmul."""
-    what = "residual_norm_fwd"
-    px, sx = _lib.rows_ptr(x, f"{what}: x", (_BF, _F32))
+    px, sx = _lib.rows_ptr(x, "residual_norm_fwd: x", (_BF, _F32))
     rows, d = x.shape
-    ph, sh = _lib.rows_ptr(h, f"{what}: h", (_BF, _F32), d)
+    ph, sh = _lib.rows_ptr(h, "residual_norm_fwd: h", (_BF, _F32), d)
     if h.shape[0] != rows or not 1 <= d <= 8192 or z_dtype not in (_BF, _F32) or (pack and pre is None):
-        raise _lib.SwatHipError(f"{what}: x {tuple(x.shape)}, h {tuple(h.shape)} (the same rows, 1 to 8192 columns), z in bf16 or fp32, "
-                                "pack goes with pre")
-    pw, pb, g, groups, channels, sc, qw, qb, rms = _seam(what, rows, d, post, pre, gate, scale, norm)
-    dev = x.device
-    y = torch.empty((rows, d), dtype=x.dtype, device=dev)
-    z = torch.empty((rows, d), dtype=z_dtype, device=dev) if pre is not None else None
-    stats = torch.empty((4, rows), dtype=_F32, device=dev)
+        raise _lib.SwatHipError(f"residual_norm_fwd: x {tuple(x.shape)}, h {tuple(h.shape)} (the same rows, 1 to 8192 columns), z in bf16 or "
+                                "fp32, pack goes with pre")
+    v = _seam("residual_norm_fwd", rows, d, post, pre, gate, scale, norm)
+    y = x.new_empty((rows, d))
+    z = x.new_empty((rows, d), dtype=z_dtype) if pre is not None else None
+    stats = x.new_empty((4, rows), dtype=_F32)
     z8 = None
     if pack:
         from . import mx
-        z8 = mx._empty(rows, d, 8, dev)
-    rc = _lib.lib().swat_residual_norm_fwd(px, sx, int(x.dtype == _BF), ph, sh, int(h.dtype == _BF), pw, pb, g, groups, channels, sc, qw, qb,
-                                           float(alpha), rms, float(eps), _p(y), _p(z), int(z_dtype == _BF), _p(z8.codes) if pack else None,
-                                           _p(z8.scale) if pack else None, _p(stats), rows, d, _lib.stream())
+        z8 = mx._empty(x, rows, d, 8)
+    rc = _lib.lib().swat_residual_norm_fwd(px, sx, x.dtype == _BF, ph, sh, h.dtype == _BF, *v[:8], float(alpha), v[8], float(eps), y.data_ptr(),
+                                           z.data_ptr() if z is not None else None, z_dtype == _BF, z8.codes.data_ptr() if pack else None,
+                                           z8.scale.data_ptr() if pack else None, stats.data_ptr(), rows, d, _lib.stream())
     _chk(rc, "swat_residual_norm_fwd")
     return ResidualNorm(y, z, stats, z8)
 
@@ -155,33 +154,38 @@ def residual_norm_fwd(x, h, post=None, pre=None, gate=None, scale=None, alpha=1.
 def residual_norm_bwd(dy, dz, h, y, stats, post=None, pre=None, gate=None, scale=None, alpha=1.0, norm="layer"):
     """Backward of residual_norm_fwd: dy (stream, may be None) and dz (None without pre) -> dict of gradients: 'x', 'h', and of what was
     given 'post_w', 'post_b', 'gate', 'scale', 'pre_w', 'pre_b'.  y, stats: the forward's (y may be None without pre).  Sums in a fixed order."""
-    what = "residual_norm_bwd"
-    ph, sh = _lib.rows_ptr(h, f"{what}: h", (_BF, _F32))
+    ph, sh = _lib.rows_ptr(h, "residual_norm_bwd: h", (_BF, _F32))
     rows, d = h.shape
     if (dz is None) != (pre is None) or (dy is None and dz is None) or (pre is not None and y is None) or not 1 <= d <= 8192:
-        raise _lib.SwatHipError(f"{what}: dz and y go with pre, dy or dz is needed, 1 to 8192 columns (d = {d})")
+        raise _lib.SwatHipError(f"residual_norm_bwd: dz and y go with pre, dy or dz is needed, 1 to 8192 columns (d = {d})")
     xt = y.dtype if y is not None else dy.dtype
-    pdy, sdy = _lib.rows_ptr(dy, f"{what}: dy", (xt,), d) if dy is not None else (None, d)
-    pdz, sdz = _lib.rows_ptr(dz, f"{what}: dz", (_BF, _F32), d) if dz is not None else (None, d)
-    py, sy = _lib.rows_ptr(y, f"{what}: y", (_BF, _F32), d) if y is not None else (None, d)
-    if xt not in (_BF, _F32) or any(t is not None and t.shape[0] != rows for t in (dy, dz, y)):
-        raise _lib.SwatHipError(f"{what}: dy, dz, h and y have the same rows; the stream is bf16 or fp32")
-    pst = _lib.vec_ptr(stats, f"{what}: stats", (4, rows))
-    pw, pb, g, groups, channels, sc, qw, qb, rms = _seam(what, rows, d, post, pre, gate, scale, norm)
-    dev = h.device
-    out = {"x": torch.empty((rows, d), dtype=xt, device=dev), "h": torch.empty((rows, d), dtype=h.dtype, device=dev)}
-    for name, t in (("post_w", pw), ("post_b", pb), ("scale", sc), ("pre_w", qw), ("pre_b", qb)):
-        if t is not None:
-            out[name] = torch.empty(d, dtype=_F32, device=dev)
-    if gate is not None:
+    pdy, sdy = _lib.rows_ptr(dy, "residual_norm_bwd: dy", (xt,), d) if dy is not None else (None, d)
+    pdz, sdz = _lib.rows_ptr(dz, "residual_norm_bwd: dz", (_BF, _F32), d) if dz is not None else (None, d)
+    py, sy = _lib.rows_ptr(y, "residual_norm_bwd: y", (_BF, _F32), d) if y is not None else (None, d)
+    if (xt != _BF and xt != _F32) or any(t is not None and t.shape[0] != rows for t in (dy, dz, y)):
+        raise _lib.SwatHipError("residual_norm_bwd: dy, dz, h and y have the same rows; the stream is bf16 or fp32")
+    pst = _lib.vec_ptr(stats, "residual_norm_bwd: stats", 4, rows)
+    v = _seam("residual_norm_bwd", rows, d, post, pre, gate, scale, norm)
+    pw, pb, g, groups, channels, sc, qw, qb, rms = v
+    out = {"x": h.new_empty((rows, d), dtype=xt), "h": h.new_empty((rows, d))}
+    names = [n for n, t in (("post_w", pw), ("post_b", pb), ("scale", sc), ("pre_w", qw), ("pre_b", qb)) if t is not None]
+    cols = {}
+    if names:  # (one allocation: a row each)
+        flat = h.new_empty((len(names), d), dtype=_F32)
+        base = flat.data_ptr()
+        for i, (n, t) in enumerate(zip(names, flat.unbind(0))):
+            out[n] = t
+            cols[n] = base + 4 * d * i
+    dgate = None
+    if g is not None:
         out["gate"] = torch.empty_like(gate)
-    nbytes = _lib.lib().swat_residual_norm_bwd_workspace_bytes(rows, d, groups, channels)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    rc = _lib.lib().swat_residual_norm_bwd(pdy, sdy, pdz, sdz, int(dz is not None and dz.dtype == _BF), ph, sh, int(h.dtype == _BF), py, sy,
-                                           int(xt == _BF), pst, pw, pb, g, groups, channels, sc, qw, qb, float(alpha), rms, _p(out["x"]),
-                                           _p(out["h"]), _p(out.get("post_w")), _p(out.get("post_b")), _p(out.get("gate")),
-                                           _p(out.get("scale")), _p(out.get("pre_w")), _p(out.get("pre_b")), _p(ws), nbytes, rows, d,
-                                           _lib.stream())
+        dgate = out["gate"].data_ptr()
+    h_ = _lib.lib()
+    nbytes = h_.swat_residual_norm_bwd_workspace_bytes(rows, d, groups, channels)
+    ws = h.new_empty(nbytes, dtype=torch.uint8)
+    rc = h_.swat_residual_norm_bwd(pdy, sdy, pdz, sdz, dz is not None and dz.dtype == _BF, ph, sh, h.dtype == _BF, py, sy, xt == _BF, pst,
+                                   *v[:8], float(alpha), rms, out["x"].data_ptr(), out["h"].data_ptr(), cols.get("post_w"), cols.get("post_b"),
+                                   dgate, cols.get("scale"), cols.get("pre_w"), cols.get("pre_b"), ws.data_ptr(), nbytes, rows, d, _lib.stream())
     _chk(rc, "swat_residual_norm_bwd")
     return out
 
