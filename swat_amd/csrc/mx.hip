@@ -7,7 +7,7 @@
 // Storage: codes [rows, n rounded up to 32] (8 bits) or half of that (4 bits, the even column in the low half), scales
 // [rows, blocks of 32]; the columns behind n hold zeros, so every row starts on 32 (16) bytes and products need no edge along them.
 //
-// All of them are bound by bytes.  A thread takes 8 neighbouring columns (16 bytes of bfloat16, 8 or 4 of codes), four lanes make
+// All of them are bound by bytes (8224 x 4096 there and back 5.5 and 6.3 TB/s; 16448 x 1024 fp32 to 4 bits 12.5 us, back 14.7).  A thread takes 8 neighbouring columns (16 bytes of bfloat16, 8 or 4 of codes), four lanes make
 // a block and agree on its scale by two lane exchanges.
 #include "gemm_device.hpp"
 #include "mx_device.hpp"
@@ -15,13 +15,16 @@
 
 namespace swat {
 
-// column chunk of 8 <-> thread: chunks per row is a multiple of 4; q = floor(idx / cpr) by multiplication (mul = ceil(2^(32+sh) / cpr))
+// chunks of 8 columns, a multiple of 4 to a row; a thread takes one
 struct MxMap {
     int64_t rows;
     int n, blocks;        // columns; blocks of 32 to a row
     int64_t ld;           // row stride of the values read (elements)
-    int vec;              // values and outputs sit on 16-byte rows and n % 8 == 0
 };
+
+// vectors at any element's address (rows of odd widths)
+typedef unsigned mx_u4h __attribute__((ext_vector_type(4), aligned(2)));
+typedef unsigned mx_u4f __attribute__((ext_vector_type(4), aligned(4)));
 
 __device__ __forceinline__ bool mx_place(const MxMap& m, int64_t& row, int& col) {
     const unsigned cpr = 4u * (unsigned)m.blocks;
@@ -37,35 +40,43 @@ __device__ __forceinline__ bool mx_place(const MxMap& m, int64_t& row, int& col)
     return row < m.rows;
 }
 
-__device__ __forceinline__ void mx_load8(const void* p, int bf, int64_t at, int left, bool vec, float (&v)[8]) {
-    if (vec && left >= 8) {
+__device__ __forceinline__ void mx_load8(const void* p, int bf, int64_t at, int left, float (&v)[8]) {
+    if (left >= 8) {
         if (bf) {
-            const uint4 u = *reinterpret_cast<const uint4*>(reinterpret_cast<const unsigned short*>(p) + at);
-            const unsigned w[4] = {u.x, u.y, u.z, u.w};
+            const mx_u4h u = *reinterpret_cast<const mx_u4h*>(reinterpret_cast<const unsigned short*>(p) + at);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                v[2 * i] = __uint_as_float(w[i] << 16);
-                v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+                v[2 * i] = __uint_as_float(u[i] << 16);
+                v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
             }
         } else {
-            const float4 a = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + at);
-            const float4 b = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + at + 4);
-            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-            v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+            const mx_u4f a = *reinterpret_cast<const mx_u4f*>(reinterpret_cast<const float*>(p) + at);
+            const mx_u4f b = *reinterpret_cast<const mx_u4f*>(reinterpret_cast<const float*>(p) + at + 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v[i] = __uint_as_float(a[i]);
+                v[4 + i] = __uint_as_float(b[i]);
+            }
         }
         return;
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = i >= left ? 0.f : bf ? bf2f(reinterpret_cast<const unsigned short*>(p)[at + i]) : reinterpret_cast<const float*>(p)[at + i];
 }
-__device__ __forceinline__ void mx_store8(void* p, int bf, int64_t at, int left, bool vec, const float (&v)[8]) {
-    if (vec && left >= 8) {
+__device__ __forceinline__ void mx_store8(void* p, int bf, int64_t at, int left, const float (&v)[8]) {
+    if (left >= 8) {
         if (bf) {
-            *reinterpret_cast<uint4*>(reinterpret_cast<unsigned short*>(p) + at) =
-                make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+            *reinterpret_cast<mx_u4h*>(reinterpret_cast<unsigned short*>(p) + at) =
+                (mx_u4h){pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
         } else {
-            *reinterpret_cast<float4*>(reinterpret_cast<float*>(p) + at) = make_float4(v[0], v[1], v[2], v[3]);
-            *reinterpret_cast<float4*>(reinterpret_cast<float*>(p) + at + 4) = make_float4(v[4], v[5], v[6], v[7]);
+            mx_u4f a, b;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                a[i] = __float_as_uint(v[i]);
+                b[i] = __float_as_uint(v[4 + i]);
+            }
+            *reinterpret_cast<mx_u4f*>(reinterpret_cast<float*>(p) + at) = a;
+            *reinterpret_cast<mx_u4f*>(reinterpret_cast<float*>(p) + at + 4) = b;
         }
         return;
     }
@@ -118,7 +129,7 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(MxMap m, const void* x
     int col;
     if (!mx_place(m, row, col)) return;
     float v[8];
-    mx_load8(x, bf, row * m.ld + col, m.n - col, m.vec, v);
+    mx_load8(x, bf, row * m.ld + col, m.n - col, v);
     mx_pack8<BITS>(v, row, col, m, codes, scales);
 }
 
@@ -129,7 +140,26 @@ __global__ __launch_bounds__(256) void mx_dequantize_kernel(MxMap m, const unsig
     if (!mx_place(m, row, col) || col >= m.n) return;
     float v[8];
     mx_unpack8<BITS>(codes, scales, row, col, m, v);
-    mx_store8(out, bf, row * m.n + col, m.n - col, m.vec, v);
+    mx_store8(out, bf, row * m.n + col, m.n - col, v);
+}
+
+// act(x) and act'(x).  GELU: the normal distribution's tail by Abramowitz & Stegun 7.1.26, erfc(z) = (a1 t + .. + a5 t^5) exp(-z^2),
+// t = 1 / (1 + p z), off by 1.5e-7 at most (a bfloat16 result shows 2e-3); its exponential is the density's that the slope needs as well,
+// so one exponential and one reciprocal serve both (8224 x 4096, with the library's erf: forward 37 us, backward 60, bound by arithmetic;
+// so 31 and 38, bound by bytes).
+__device__ __forceinline__ void mx_act(float x, int act, float& value, float& slope) {
+    if (act == 1) {
+        const float s = __builtin_amdgcn_rcpf(1.0f + __expf(-1.702f * x));
+        value = x * s;
+        slope = s * (1.0f + 1.702f * x * (1.0f - s));
+        return;
+    }
+    const float z = fabsf(x) * 0.70710678118654752f, e = __expf(-0.5f * x * x);
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, z, 1.0f));
+    const float poly = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+    const float tail = 0.5f * poly * e, cdf = x < 0.f ? tail : 1.0f - tail;
+    value = x * cdf;
+    slope = fmaf(x * 0.39894228040143268f, e, cdf);
 }
 
 __global__ __launch_bounds__(256) void mx_act_fwd_kernel(MxMap m, const unsigned short* f, int act, unsigned short* g, unsigned char* codes, unsigned char* scales) {
@@ -137,10 +167,13 @@ __global__ __launch_bounds__(256) void mx_act_fwd_kernel(MxMap m, const unsigned
     int col;
     if (!mx_place(m, row, col)) return;
     float v[8], t[8];
-    mx_load8(f, 1, row * m.ld + col, m.n - col, m.vec, v);
+    mx_load8(f, 1, row * m.ld + col, m.n - col, v);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) t[i] = act_fwd(v[i], act);
-    mx_store8(g, 1, row * m.n + col, m.n - col, m.vec, t);
+    for (int i = 0; i < 8; ++i) {
+        float slope;
+        mx_act(v[i], act, t[i], slope);
+    }
+    mx_store8(g, 1, row * m.n + col, m.n - col, t);
     mx_pack8<8>(v, row, col, m, codes, scales);
 }
 
@@ -150,28 +183,28 @@ __global__ __launch_bounds__(256) void mx_act_bwd_kernel(MxMap m, const unsigned
     int col;
     if (!mx_place(m, row, col) || col >= m.n) return;
     float v[8], t[8];
-    mx_load8(dg, 1, row * m.ld + col, m.n - col, m.vec, t);
+    mx_load8(dg, 1, row * m.ld + col, m.n - col, t);
     mx_unpack8<8>(codes, scales, row, col, m, v);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) t[i] *= act_bwd(v[i], act);
-    mx_store8(df, 1, row * m.n + col, m.n - col, m.vec, t);
-    if (again) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = act_fwd(v[i], act);
-        mx_store8(again, 1, row * m.n + col, m.n - col, m.vec, v);
+    for (int i = 0; i < 8; ++i) {
+        float value, slope;
+        mx_act(v[i], act, value, slope);
+        t[i] *= slope;
+        v[i] = value;
     }
+    mx_store8(df, 1, row * m.n + col, m.n - col, t);
+    if (again) mx_store8(again, 1, row * m.n + col, m.n - col, v);
 }
 
 static bool on16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 // columns of one row at most: 4 (n / 32) chunk indexes and 8 of them to a thread stay in 32 bits
-static int mx_map(MxMap& m, int64_t rows, int n, int64_t ld, int in_bytes, const char* what) {
+static int mx_map(MxMap& m, int64_t rows, int n, int64_t ld, const char* what) {
     SWAT_REQUIRE(rows >= 0 && n >= 1 && n <= (1 << 24), "%s: %lld rows of %d columns (0 or more rows, 1 to 2^24 columns)", what, (long long)rows, n);
     SWAT_REQUIRE(ld >= n, "%s: row stride %lld under %d columns", what, (long long)ld, n);
     m.rows = rows;
     m.n = n;
     m.blocks = (n + 31) / 32;
     m.ld = ld;
-    m.vec = n % 8 == 0 && ld * in_bytes % 16 == 0;
     SWAT_REQUIRE(rows * (4 * (int64_t)m.blocks) <= ((int64_t)1 << 39), "%s: %lld rows of %d columns are past one launch", what, (long long)rows, n);
     return 0;
 }
@@ -186,10 +219,9 @@ SWAT_API int swat_mx_quantize(const void* x, int64_t x_stride, int x_dtype, int 
     MxMap m;
     const int bf = x_dtype == SWAT_BF16;
     SWAT_REQUIRE(bits == 4 || bits == 8, "swat_mx_quantize: %d bits (4 or 8)", bits);
-    if (const int rc = mx_map(m, rows, n, x_stride, bf ? 2 : 4, "swat_mx_quantize")) return rc;
+    if (const int rc = mx_map(m, rows, n, x_stride, "swat_mx_quantize")) return rc;
     if (rows == 0) return 0;
     SWAT_REQUIRE(x && codes && scales && on16(codes), "swat_mx_quantize: x, codes (on 16 bytes) and scales are needed");
-    m.vec = m.vec && on16(x);
     unsigned char *c = (unsigned char*)codes, *s = (unsigned char*)scales;
     if (bits == 8) mx_quantize_kernel<8><<<mx_grid(m), 256, 0, (hipStream_t)stream>>>(m, x, bf, c, s);
     else mx_quantize_kernel<4><<<mx_grid(m), 256, 0, (hipStream_t)stream>>>(m, x, bf, c, s);
@@ -201,10 +233,9 @@ SWAT_API int swat_mx_dequantize(const void* codes, const void* scales, int bits,
     MxMap m;
     const int bf = out_dtype == SWAT_BF16;
     SWAT_REQUIRE(bits == 4 || bits == 8, "swat_mx_dequantize: %d bits (4 or 8)", bits);
-    if (const int rc = mx_map(m, rows, n, n, bf ? 2 : 4, "swat_mx_dequantize")) return rc;
+    if (const int rc = mx_map(m, rows, n, n, "swat_mx_dequantize")) return rc;
     if (rows == 0) return 0;
     SWAT_REQUIRE(out && codes && scales && on16(codes), "swat_mx_dequantize: out, codes (on 16 bytes) and scales are needed");
-    m.vec = m.vec && on16(out);
     const unsigned char *c = (const unsigned char*)codes, *s = (const unsigned char*)scales;
     if (bits == 8) mx_dequantize_kernel<8><<<mx_grid(m), 256, 0, (hipStream_t)stream>>>(m, c, s, out, bf);
     else mx_dequantize_kernel<4><<<mx_grid(m), 256, 0, (hipStream_t)stream>>>(m, c, s, out, bf);
@@ -215,10 +246,9 @@ SWAT_API int swat_mx_act_fwd(const void* f_bf16, int64_t f_stride, int act, void
                              swat_stream_t stream) {
     MxMap m;
     SWAT_REQUIRE(act == 1 || act == 2, "swat_mx_act_fwd: activation %d (1 QuickGELU, 2 erf-GELU)", act);
-    if (const int rc = mx_map(m, rows, n, f_stride, 2, "swat_mx_act_fwd")) return rc;
+    if (const int rc = mx_map(m, rows, n, f_stride, "swat_mx_act_fwd")) return rc;
     if (rows == 0) return 0;
     SWAT_REQUIRE(f_bf16 && g_bf16 && codes && scales && on16(codes), "swat_mx_act_fwd: f, g, codes (on 16 bytes) and scales are needed");
-    m.vec = m.vec && on16(f_bf16) && on16(g_bf16);
     mx_act_fwd_kernel<<<mx_grid(m), 256, 0, (hipStream_t)stream>>>(m, (const unsigned short*)f_bf16, act, (unsigned short*)g_bf16, (unsigned char*)codes, (unsigned char*)scales);
     return check_launch("swat_mx_act_fwd");
 }
@@ -227,10 +257,9 @@ SWAT_API int swat_mx_act_bwd(const void* dg_bf16, int64_t dg_stride, const void*
                              int64_t rows, int n, swat_stream_t stream) {
     MxMap m;
     SWAT_REQUIRE(act == 1 || act == 2, "swat_mx_act_bwd: activation %d (1 QuickGELU, 2 erf-GELU)", act);
-    if (const int rc = mx_map(m, rows, n, dg_stride, 2, "swat_mx_act_bwd")) return rc;
+    if (const int rc = mx_map(m, rows, n, dg_stride, "swat_mx_act_bwd")) return rc;
     if (rows == 0) return 0;
     SWAT_REQUIRE(dg_bf16 && df_bf16 && codes && scales && on16(codes), "swat_mx_act_bwd: dg, df, codes (on 16 bytes) and scales are needed");
-    m.vec = m.vec && on16(dg_bf16) && on16(df_bf16) && on16(g_bf16);
     mx_act_bwd_kernel<<<mx_grid(m), 256, 0, (hipStream_t)stream>>>(m, (const unsigned short*)dg_bf16, (const unsigned char*)codes, (const unsigned char*)scales, act,
                                                                    (unsigned short*)df_bf16, (unsigned short*)g_bf16);
     return check_launch("swat_mx_act_bwd");
