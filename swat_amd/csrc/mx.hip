@@ -40,18 +40,19 @@ __device__ __forceinline__ bool mx_place(const MxMap& m, int64_t& row, int& col)
     return row < m.rows;
 }
 
+// (read once by a call: non-temporal, the caches are left to what is written and to the packed form)
 __device__ __forceinline__ void mx_load8(const void* p, int bf, int64_t at, int left, float (&v)[8]) {
     if (left >= 8) {
         if (bf) {
-            const mx_u4h u = *reinterpret_cast<const mx_u4h*>(reinterpret_cast<const unsigned short*>(p) + at);
+            const mx_u4h u = __builtin_nontemporal_load(reinterpret_cast<const mx_u4h*>(reinterpret_cast<const unsigned short*>(p) + at));
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 v[2 * i] = __uint_as_float(u[i] << 16);
                 v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
             }
         } else {
-            const mx_u4f a = *reinterpret_cast<const mx_u4f*>(reinterpret_cast<const float*>(p) + at);
-            const mx_u4f b = *reinterpret_cast<const mx_u4f*>(reinterpret_cast<const float*>(p) + at + 4);
+            const mx_u4f a = __builtin_nontemporal_load(reinterpret_cast<const mx_u4f*>(reinterpret_cast<const float*>(p) + at));
+            const mx_u4f b = __builtin_nontemporal_load(reinterpret_cast<const mx_u4f*>(reinterpret_cast<const float*>(p) + at + 4));
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 v[i] = __uint_as_float(a[i]);
