@@ -28,7 +28,7 @@ typedef unsigned mx_u4f __attribute__((ext_vector_type(4), aligned(4)));
 
 __device__ __forceinline__ bool mx_place(const MxMap& m, int64_t& row, int& col) {
     const unsigned cpr = 4u * (unsigned)m.blocks;
-    const int64_t idx = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    const int64_t idx = mx_block() * blockDim.x + threadIdx.x;
     if (idx < 0x7fffffff) {
         const unsigned i = (unsigned)idx, r = i / cpr;
         row = r;
@@ -209,7 +209,7 @@ static int mx_map(MxMap& m, int64_t rows, int n, int64_t ld, const char* what) {
     SWAT_REQUIRE(rows * (4 * (int64_t)m.blocks) <= ((int64_t)1 << 39), "%s: %lld rows of %d columns are past one launch", what, (long long)rows, n);
     return 0;
 }
-static unsigned mx_grid(const MxMap& m) { return (unsigned)((m.rows * 4 * m.blocks + 255) / 256); }
+static dim3 mx_grid(const MxMap& m) { return mx_grid2((m.rows * 4 * m.blocks + 255) / 256); }
 
 }  // namespace swat
 

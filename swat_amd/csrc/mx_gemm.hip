@@ -355,21 +355,26 @@ __global__ __launch_bounds__(512, 2) void mx_rows_kernel(MxGemmArgs p) {
 }
 
 template <int AB, int BB>
-static void mx_rows(MxGemmArgs p, int64_t m_begin, int rows, hipStream_t s) {
+static bool mx_rows(MxGemmArgs p, int64_t m_begin, int rows, hipStream_t s) {
     // a workgroup to each 16-row part while they stay within 2 to a CU (64 rows, 4 bits, k 4096: 1024 columns 5.7 us with 256 workgroups,
     // 10.9 with 64; k 1024: 4096 columns 5.8 with 1024, 4.8 with 256)
     p.m_begin = (int)m_begin;
     p.tiles_n = (int)((p.N + 15) / 16);
-    const int parts = (rows + 15) / 16;
-    if ((int64_t)p.tiles_n * parts <= 512) mx_rows_kernel<AB, BB, 1><<<(unsigned)(p.tiles_n * parts), 512, 0, s>>>(p);
-    else mx_rows_kernel<AB, BB, 4><<<(unsigned)(p.tiles_n * ((parts + 3) / 4)), 512, 0, s>>>(p);
+    const int64_t parts = (rows + 15) / 16, few = p.tiles_n * parts, many = p.tiles_n * ((parts + 3) / 4);
+    if (many >= 1 << 23) return false;   // (2^32 threads)
+    if (few <= 512) mx_rows_kernel<AB, BB, 1><<<(unsigned)few, 512, 0, s>>>(p);
+    else mx_rows_kernel<AB, BB, 4><<<(unsigned)many, 512, 0, s>>>(p);
+    return true;
 }
 template <int AB, int BB, int BM, int BN, int WM, int WN>
-static void mx_tiles(MxGemmArgs p, int64_t rows, hipStream_t s) {
+static bool mx_tiles(MxGemmArgs p, int64_t rows, hipStream_t s) {
     p.M = rows;   // (rows behind them, if any, go to mx_rows)
     p.tiles_m = (int)((rows + BM - 1) / BM);
     p.tiles_n = (int)((p.N + BN - 1) / BN);
-    mx_gemm_kernel<AB, BB, BM, BN, WM, WN><<<(unsigned)(p.tiles_m * p.tiles_n), (BM / WM) * (BN / WN) * 64, 0, s>>>(p);
+    const int64_t grid = (int64_t)p.tiles_m * p.tiles_n;
+    if (grid >= 1 << 23) return false;
+    mx_gemm_kernel<AB, BB, BM, BN, WM, WN><<<(unsigned)grid, (BM / WM) * (BN / WN) * 64, 0, s>>>(p);
+    return true;
 }
 
 // Which tile, by the sum of what was measured (us, 4 by 4 bits; an 8-bit operand adds 28 %): a 128-column step takes a CU 0.8 with five
@@ -412,12 +417,13 @@ static MxGemmPlan mx_plan(int64_t M, int64_t N, int blocks, int ab, int bb) {
     return best;
 }
 template <int AB, int BB>
-static void mx_product(const MxGemmArgs& p, hipStream_t s) {
+static bool mx_product(const MxGemmArgs& p, hipStream_t s) {
     const MxGemmPlan pl = mx_plan(p.M, p.N, p.blocks, AB, BB);
-    if (pl.size == 1) mx_tiles<AB, BB, 64, 64, 32, 32>(p, pl.rows, s);
-    else if (pl.size == 2) mx_tiles<AB, BB, 128, 128, 64, 64>(p, pl.rows, s);
-    else if (pl.size == 3) mx_tiles<AB, BB, 256, 256, 128, 64>(p, pl.rows, s);
-    for (int64_t m = pl.rows; m < p.M; m += 64) mx_rows<AB, BB>(p, m, p.M - m < 64 ? (int)(p.M - m) : 64, s);
+    const bool ok = pl.size == 1   ? mx_tiles<AB, BB, 64, 64, 32, 32>(p, pl.rows, s)
+                    : pl.size == 2 ? mx_tiles<AB, BB, 128, 128, 64, 64>(p, pl.rows, s)
+                    : pl.size == 3 ? mx_tiles<AB, BB, 256, 256, 128, 64>(p, pl.rows, s)
+                                   : true;
+    return ok && (pl.rows == p.M || mx_rows<AB, BB>(p, pl.rows, (int)(p.M - pl.rows), s));
 }
 
 }  // namespace swat
@@ -427,7 +433,7 @@ using namespace swat;
 SWAT_API int swat_mx_matmul(const void* a_codes, const void* a_scales, int a_bits, const void* b_codes, const void* b_scales, int b_bits,
                             const float* bias, void* c, int c_dtype, int64_t M, int64_t N, int K, swat_stream_t stream) {
     SWAT_REQUIRE((a_bits == 4 || a_bits == 8) && (b_bits == 4 || b_bits == 8), "swat_mx_matmul: %d and %d bits (4 or 8 each)", a_bits, b_bits);
-    SWAT_REQUIRE(M >= 0 && N >= 0 && K >= 1 && K <= (1 << 22) && M < (1ll << 31) && N < (1ll << 31), "swat_mx_matmul: %lld x %lld x %d", (long long)M, (long long)N, K);
+    SWAT_REQUIRE(M >= 0 && N >= 0 && K >= 1 && K <= (1 << 22) && M <= (1 << 30) && N <= (1 << 30), "swat_mx_matmul: %lld x %lld x %d", (long long)M, (long long)N, K);
     SWAT_REQUIRE(c_dtype == SWAT_BF16 || (c_dtype == SWAT_F32 && a_bits == 4 && b_bits == 4), "swat_mx_matmul: output type %d of %d by %d bits (bf16; fp32 where both have 4 bits)", c_dtype, a_bits, b_bits);
     if (M == 0 || N == 0) return 0;
     SWAT_REQUIRE(a_codes && a_scales && b_codes && b_scales && c, "swat_mx_matmul: both operands and the output are needed");
@@ -436,9 +442,8 @@ SWAT_API int swat_mx_matmul(const void* a_codes, const void* a_scales, int a_bit
     p.A = (const unsigned char*)a_codes; p.sA = (const unsigned char*)a_scales; p.B = (const unsigned char*)b_codes; p.sB = (const unsigned char*)b_scales;
     p.bias = bias; p.C = c; p.M = M; p.N = N; p.blocks = (K + 31) / 32; p.out_bf = c_dtype == SWAT_BF16;
     const hipStream_t s = (hipStream_t)stream;
-    if (a_bits == 4 && b_bits == 4) mx_product<4, 4>(p, s);
-    else if (a_bits == 8 && b_bits == 4) mx_product<8, 4>(p, s);
-    else if (a_bits == 4 && b_bits == 8) mx_product<4, 8>(p, s);
-    else mx_product<8, 8>(p, s);
+    const bool ok = a_bits == 4 ? (b_bits == 4 ? mx_product<4, 4>(p, s) : mx_product<4, 8>(p, s))
+                                : (b_bits == 4 ? mx_product<8, 4>(p, s) : mx_product<8, 8>(p, s));
+    SWAT_REQUIRE(ok, "swat_mx_matmul: %lld x %lld is past one launch", (long long)M, (long long)N);
     return check_launch("swat_mx_matmul");
 }

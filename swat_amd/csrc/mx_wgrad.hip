@@ -319,7 +319,7 @@ SWAT_API int swat_mx_linear_wgrad(const void* dY_bf16, int64_t dy_stride, const 
     SWAT_REQUIRE(!(((uintptr_t)x_codes | (uintptr_t)dW) & 15), "swat_mx_linear_wgrad: codes and dW sit on 16 bytes");
     const MxWgradPlan pl = mx_wgrad_plan(rows, n_out, n_in);
     const int64_t grid = (int64_t)pl.tiles_n * pl.tiles_k * pl.splits, nk = (int64_t)n_out * n_in;
-    SWAT_REQUIRE(grid < (1ll << 31) && nk < (1ll << 40), "swat_mx_linear_wgrad: %d x %d is past one launch", n_out, n_in);
+    SWAT_REQUIRE(grid < (1ll << 23) && nk < (1ll << 34), "swat_mx_linear_wgrad: %d x %d is past one launch", n_out, n_in);
     const int64_t want = swat_mx_linear_wgrad_workspace_bytes(rows, n_out, n_in);
     SWAT_REQUIRE(want == 0 || (workspace && workspace_bytes >= want && ((uintptr_t)workspace & 15) == 0),
                  "swat_mx_linear_wgrad: workspace of %lld bytes, %lld on 16 bytes are needed", (long long)workspace_bytes, (long long)want);

@@ -195,7 +195,7 @@ template <int W, int NCH>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void residual_norm_fwd_kernel(RnArgs a) {
     __shared__ float sh[W];
     const int lane = threadIdx.x & (64 * W - 1);
-    const int64_t row = W == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+    const int64_t row = W == 1 ? mx_block() * 4 + (threadIdx.x >> 6) : mx_block();
     if (row >= a.rows) return;
     const int d = a.d, c0 = lane * 4;
     constexpr int STEP = 256 * W;
@@ -643,6 +643,7 @@ static bool rn_try(const RnPlan& p, F&& launch) {   // W and one of N vectors to
 static int rn_common(RnArgs& a, int rows, int d, int64_t groups, int gate_channels, const char* what) {
     SWAT_REQUIRE(rows >= 0 && d >= 1 && d <= 8192, "%s: rows %d, width %d (0 rows or more, 1 to 8192 columns)", what, rows, d);
     SWAT_REQUIRE(!a.gate || (groups >= 1 && rows % groups == 0), "%s: %lld gates do not divide %d rows", what, (long long)groups, rows);
+    SWAT_REQUIRE(!a.gate || groups == rows || groups < (1 << 25) / (gate_channels ? 4 * ((d + 255) / 256) : 1), "%s: %lld gates are past one launch", what, (long long)groups);
     SWAT_REQUIRE((a.post_w || !a.post_b) && (a.pre_w || !a.pre_b), "%s: a norm's bias without its weight", what);
     a.rows = rows;
     a.d = d;
@@ -679,7 +680,7 @@ SWAT_API int swat_residual_norm_fwd(const void* x, int64_t x_stride, int x_dtype
     const RnPlan p = rn_plan(rows, d, false);
     auto go = [&](auto w, auto n) {
         constexpr int W = decltype(w)::value, N = decltype(n)::value;
-        residual_norm_fwd_kernel<W, N><<<W == 1 ? (rows + 3) / 4 : rows, W == 1 ? 256 : 64 * W, 0, (hipStream_t)stream>>>(a);
+        residual_norm_fwd_kernel<W, N><<<mx_grid2(W == 1 ? ((int64_t)rows + 3) / 4 : rows), W == 1 ? 256 : 64 * W, 0, (hipStream_t)stream>>>(a);
     };
     SWAT_REQUIRE((rn_try<1, 1, 2, 3, 4>(p, go) || rn_try<4, 2, 4>(p, go) || rn_try<8, 4>(p, go)), "swat_residual_norm_fwd: no kernel for %d columns", d);
     return check_launch("swat_residual_norm_fwd");

@@ -13,6 +13,7 @@ from . import _lib
 from .ops import ACT
 
 _BF, _F32 = torch.bfloat16, torch.float32
+_COLS = 1 << 24  # columns of a matrix at most (the C entries take them as 32-bit numbers)
 
 
 class MX(namedtuple("MX", "codes scale cols bits")):
@@ -36,8 +37,8 @@ def _empty(like, rows, cols, bits):
 
 def _check(m, what, bits=(4, 8)):
     """The pointers of an MX matrix whose parts fit together, on the current device."""
-    if not isinstance(m, MX) or m.bits not in bits or m.cols < 1:
-        raise _lib.SwatHipError(f"{what}: an MX matrix of {' or '.join(map(str, bits))} bits is wanted, got {m!r:.80}")
+    if not isinstance(m, MX) or m.bits not in bits or not 1 <= m.cols <= _COLS:
+        raise _lib.SwatHipError(f"{what}: an MX matrix of {' or '.join(map(str, bits))} bits and 1 to {_COLS} columns is wanted, got {m!r:.80}")
     codes, scale = m.codes, m.scale
     rows, blocks = codes.shape[0], (m.cols + 31) // 32
     if (codes.dtype != torch.uint8 or scale.dtype != torch.uint8 or codes.shape != (rows, blocks * 4 * m.bits) or scale.shape != (rows, blocks)
@@ -58,8 +59,8 @@ def _act(act, what):
 def quantize(x, bits=8):
     """x [rows, cols] bf16 or fp32 (rows may be strided) -> MX."""
     px, ld = _lib.rows_ptr(x, "mx.quantize", (_BF, _F32))
-    if bits not in (4, 8) or x.shape[1] < 1:
-        raise _lib.SwatHipError(f"mx.quantize: {bits} bits (4 or 8) of {x.shape[1]} columns (1 at least)")
+    if bits not in (4, 8) or not 1 <= x.shape[1] <= _COLS:
+        raise _lib.SwatHipError(f"mx.quantize: {bits} bits (4 or 8) of {x.shape[1]} columns (1 to {_COLS})")
     m = _empty(x, x.shape[0], x.shape[1], bits)
     _lib.check(_lib.lib().swat_mx_quantize(px, ld, x.dtype == _BF, bits, m.codes.data_ptr(), m.scale.data_ptr(), x.shape[0], x.shape[1],
                                            _lib.stream()), "swat_mx_quantize")
@@ -81,8 +82,8 @@ def act_fwd(f, act="gelu"):
     """f bf16 [rows, n] -> (act(f) bf16, the 8-bit checkpoint of f), f read once."""
     pf, ld = _lib.rows_ptr(f, "mx.act_fwd", (_BF,))
     a = _act(act, "mx.act_fwd")
-    if f.shape[1] < 1:
-        raise _lib.SwatHipError("mx.act_fwd: no columns")
+    if not 1 <= f.shape[1] <= _COLS:
+        raise _lib.SwatHipError(f"mx.act_fwd: {f.shape[1]} columns (1 to {_COLS})")
     m = _empty(f, f.shape[0], f.shape[1], 8)
     g = f.new_empty(f.shape)
     _lib.check(_lib.lib().swat_mx_act_fwd(pf, ld, a, g.data_ptr(), m.codes.data_ptr(), m.scale.data_ptr(), f.shape[0], f.shape[1],
@@ -109,8 +110,8 @@ def linear_wgrad(dy, m, want_bias=False, out=None):
     codes, scale = _check(m, "mx.linear_wgrad", (8,))
     py, ld = _lib.rows_ptr(dy, "mx.linear_wgrad: dy", (_BF,))
     rows, n = dy.shape
-    if rows != m.rows:
-        raise _lib.SwatHipError(f"mx.linear_wgrad: {rows} rows of dy, {m.rows} of the checkpoint")
+    if rows != m.rows or n > _COLS:
+        raise _lib.SwatHipError(f"mx.linear_wgrad: {rows} rows of {n} columns of dy, {m.rows} rows of the checkpoint")
     if out is None:
         out = dy.new_empty((n, m.cols), dtype=_F32)
     pw = _lib.vec_ptr(out, "mx.linear_wgrad: out", n, m.cols)

@@ -107,6 +107,8 @@ def _seam(what, rows, d, post, pre, gate, scale, norm):
     """The checked pointers of what both directions of the seam take: post w, b, gate, groups, per channel, scale, pre w, b, rms."""
     if norm != "layer" and norm != "rms":
         raise _lib.SwatHipError(f"{what}: norm {norm!r} ('layer' or 'rms')")
+    if rows >= 1 << 31:
+        raise _lib.SwatHipError(f"{what}: {rows} rows (under 2^31)")
     pw, pb = post if post is not None else (None, None)
     qw, qb = pre if pre is not None else (None, None)
     if (post is not None and pw is None) or (pre is not None and qw is None):
@@ -114,6 +116,8 @@ def _seam(what, rows, d, post, pre, gate, scale, norm):
     vec = _lib.vec_ptr
     g, groups, channels = None, 0, 0
     if gate is not None:
+        if gate.dim() not in (1, 2):
+            raise _lib.SwatHipError(f"{what}: gate is [groups] or [groups, d], got {tuple(gate.shape)}")
         groups, channels = gate.shape[0], int(gate.dim() == 2)
         g = vec(gate, what, groups, d) if channels else vec(gate, what, groups)
         if groups < 1 or rows % groups:

@@ -254,6 +254,33 @@ def test_packing_past_two_to_the_31_elements():
     assert not c[:-5].any()
 
 
+def test_packing_past_one_dimension_of_a_launch():
+    """2^35 elements are 2^32 threads: one more row than a launch holds along its first dimension."""
+    from swat_amd import mx
+    rows, n = 2 ** 20 + 3, 2 ** 15
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 170 << 30:
+        pytest.skip("needs 170 GB")
+    x = torch.zeros((rows, n), dtype=BF, device="cuda")
+    x[0] = rnd(n, seed=2, dtype=BF)
+    x[-5:] = rnd(5, n, seed=3, dtype=BF)
+    m = mx.quantize(x, 4)
+    for a, b in ((0, 1), (rows - 5, rows)):
+        want = mx.quantize(x[a:b], 4)
+        assert torch.equal(m.codes[a:b], want.codes) and torch.equal(m.scale[a:b], want.scale)
+    assert not m.codes[1:-5:4099].any()
+    held = mx.dequantize(mx.MX(m.codes[-5:], m.scale[-5:], n, 4))
+    out = mx.dequantize(m)
+    assert torch.equal(out[-5:], held) and not out[1:-5:4099].any()
+
+
+@pytest.mark.parametrize("abits,bbits", [(4, 4), (8, 4), (4, 8), (8, 8)])
+@pytest.mark.parametrize("M,N,K", [(100003, 3, 32), (3, 100003, 32), (5, 9000, 96), (70, 3, 160)])
+def test_product_of_few_scale_bytes(abits, bbits, M, N, K):
+    """An operand of under 16 blocks, the other long."""
+    test_product(abits, bbits, M, N, K)
+
+
 def test_a_block_trained_with_checkpoints():
     """The operators together, as a block uses them: the seam's packed z is the MLP's input checkpoint and an operand of a 4-bit product; the
     pre-activation is kept in 8 bits; the backward pass reads the checkpoints.  Captured, replayed, and against 64 bits."""

@@ -186,6 +186,24 @@ def test_rows_past_two_to_the_31_elements():
     assert not r.y[:8].any() and not r.z[rows // 2].any()
 
 
+@pytest.mark.parametrize("rows,d", [(2 ** 26 + 37, 2), (2 ** 24 + 5, 1028)])
+def test_rows_past_one_dimension_of_a_launch(rows, d):
+    """A wave (four, past 1024 columns) to a row: more than 2^32 threads."""
+    from swat_amd import ops
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 170 << 30:
+        pytest.skip("needs 170 GB")
+    x = torch.zeros((rows, d), dtype=BF, device="cuda")
+    x[:3] = rnd(3, d, seed=8, dtype=BF)
+    x[-9:] = rnd(9, d, seed=9, dtype=BF)
+    w = (rnd(d, seed=10, mean=1.0), None)
+    r = ops.residual_norm_fwd(x, x, pre=w)
+    for a, b in ((0, 3), (rows - 9, rows)):
+        want = ops.residual_norm_fwd(x[a:b], x[a:b], pre=w)
+        assert torch.equal(r.y[a:b], want.y) and torch.equal(r.z[a:b], want.z) and torch.equal(r.stats[2:, a:b], want.stats[2:]) and want.y.any()
+    assert not r.y[3:-9:40961].any() and not r.z[3:-9:40961].any()
+
+
 def test_a_captured_pass_replays():
     from swat_amd import ops
     t = make(31 * 7, 512, "layer", True, True, "group", 31, True, F32, BF, seed=70)

@@ -42,7 +42,12 @@ def test_c_entries_refuse(lib):
     refused(lib, lib.swat_mx_matmul(P, P, 4, P + 1, P, 4, None, P, 1, 4, 4, 64, None), "16 bytes")
     refused(lib, lib.swat_mx_matmul(P, P, 4, P, P, 4, None, P, 1, 4, 4, 0, None), "4 x 4")
     refused(lib, lib.swat_mx_matmul(P, P, 8, P, P, 4, None, P, 0, 4, 4, 64, None), "output type")
+    refused(lib, lib.swat_mx_matmul(P, P, 4, P, P, 4, None, P, 1, 1, (1 << 30) + 1, 64, None), "1 x 10737")
+    refused(lib, lib.swat_mx_matmul(P, P, 4, P, P, 4, None, P, 1, 1, 1 << 30, 32, None), "launch")
+    refused(lib, lib.swat_mx_matmul(P, P, 4, P, P, 4, None, P, 1, 1 << 30, 1 << 30, 64, None), "launch")
+    refused(lib, lib.swat_mx_linear_wgrad(P, 1 << 20, P, P, P, None, 64, 1 << 20, 1 << 20, None, 0, None), "launch")
     z = ctypes.c_void_p(None)
+    refused(lib, lib.swat_residual_norm_fwd(P, 16, 0, P, 16, 0, z, z, P, 1 << 25, 0, z, z, z, 1.0, 0, 1e-5, P, z, 1, z, z, z, 1 << 26, 16, None), "launch")
     refused(lib, lib.swat_residual_norm_fwd(P, 16, 0, P, 16, 0, z, z, z, 0, 0, z, z, z, 1.0, 0, 1e-5, P, z, 1, z, z, z, 4, 8193, None), "8192")
     refused(lib, lib.swat_residual_norm_fwd(P, 16, 0, P, 16, 0, z, z, P, 3, 0, z, z, z, 1.0, 0, 1e-5, P, z, 1, z, z, z, 4, 16, None), "gates")
     refused(lib, lib.swat_residual_norm_fwd(P, 15, 0, P, 16, 0, z, z, z, 0, 0, z, z, z, 1.0, 0, 1e-5, P, z, 1, z, z, z, 4, 16, None), "strides")
@@ -63,6 +68,14 @@ def test_calls_without_a_gpu_are_refused():
               lambda: ops.residual_norm_bwd(x, None, x, None, torch.zeros(4, 4))):
         with pytest.raises(_lib.SwatHipError):
             f()
+
+
+def test_more_columns_than_a_matrix_has_are_refused():
+    from swat_amd import _lib, mx
+    part = torch.zeros(1, 1, dtype=torch.uint8)
+    for cols in (0, (1 << 24) + 1, (1 << 32) + 1):   # (the last would pass as 1 in 32 bits)
+        with pytest.raises(_lib.SwatHipError, match="columns is wanted"):
+            mx.dequantize(mx.MX(part, part, cols, 8))
 
 
 def test_the_formats_of_the_formulas():
