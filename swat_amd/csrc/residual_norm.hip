@@ -455,7 +455,7 @@ __global__ __launch_bounds__(64 * W * TEAMS, 2) void residual_norm_bwd_kernel(Rn
                     const float q = g * gy[i][e];
                     cs[0][i][e] = g == 0.f ? cs[0][i][e] : fmaf(q, hat, cs[0][i][e]);
                     cs[1][i][e] += q;
-                    s[2] = c + e < d ? fmaf(sc[e] * gy[i][e], fmaf(hat, w[e], b[e]), s[2]) : s[2];
+                    s[2] = sc[e] != 0.f ? fmaf(sc[e] * gy[i][e], fmaf(hat, w[e], b[e]), s[2]) : s[2];   // (past d: zero)
                 }
                 const float v = dp * w[e];
                 s[0] += v;
@@ -498,7 +498,7 @@ __global__ __launch_bounds__(64 * W * TEAMS, 2) void residual_norm_bwd_kernel(Rn
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const float g = gate[i][e], A = cg[0][i][e], B = cg[GC][i][e];
-                        t[e] = sc[e] * fmaf(w[e], A, b[e] * B);
+                        t[e] = sc[e] == 0.f ? 0.f : sc[e] * fmaf(w[e], A, b[e] * B);
                         cs[0][i][e] = g == 0.f ? cs[0][i][e] : fmaf(g, A, cs[0][i][e]);
                         cs[1][i][e] = fmaf(g, B, cs[1][i][e]);
                         cg[0][i][e] = cg[GC][i][e] = 0.f;

@@ -159,6 +159,28 @@ def test_a_dropped_branch_may_hold_anything():
     assert torch.equal(g["gate"][live], w["gate"][live])
 
 
+@pytest.mark.parametrize("gate", ["group", "channel"])
+def test_channels_scaled_by_zero_may_hold_anything(gate):
+    """Without a norm after the sublayer: those channels enter neither the stream nor any gradient."""
+    from swat_amd import ops
+    t = make(12, 96, "layer", False, True, gate, 6, True, F32, BF, seed=65)
+    t["scale"][[0, 40, 95]] = 0.0
+    clean = t["h"].clone()
+    for c, v in ((0, float("nan")), (40, float("inf")), (95, float("-inf"))):
+        t["h"][:, c] = v
+        clean[:, c] = 0
+    kw = dict(pre=t["pre"], gate=t["gate"], scale=t["scale"])
+    a, b = (ops.residual_norm_fwd(t["x"], h, **kw) for h in (t["h"], clean))
+    assert torch.equal(a.y, b.y) and torch.equal(a.z, b.z)
+    dy, dz = rnd(12, 96, seed=66), rnd(12, 96, seed=67, dtype=BF)
+    g, w = ops.residual_norm_bwd(dy, dz, t["h"], a.y, a.stats, **kw), ops.residual_norm_bwd(dy, dz, clean, b.y, b.stats, **kw)
+    for k in g:
+        if k != "scale":  # (the scale's own gradient is what its channel holds)
+            assert torch.equal(g[k], w[k]), k
+    live = t["scale"] != 0
+    assert torch.equal(g["scale"][live], w["scale"][live])
+
+
 def test_no_rows():
     from swat_amd import ops
     t = make(0, 40, "layer", True, True, "none", 1, True, F32, BF)
