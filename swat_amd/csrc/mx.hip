@@ -20,6 +20,8 @@ struct MxMap {
     int64_t rows;
     int n, blocks;        // columns; blocks of 32 to a row
     int64_t ld;           // row stride of the values read (elements)
+    unsigned mul;         // chunk / chunks per row = chunk mul >> 32 >> shift (chunk < 2^31)
+    int shift;
 };
 
 // vectors at any element's address (rows of odd widths)
@@ -28,9 +30,9 @@ typedef unsigned mx_u4f __attribute__((ext_vector_type(4), aligned(4)));
 
 __device__ __forceinline__ bool mx_place(const MxMap& m, int64_t& row, int& col) {
     const unsigned cpr = 4u * (unsigned)m.blocks;
-    const int64_t idx = mx_block() * blockDim.x + threadIdx.x;
+    const int64_t idx = mx_block() * 256 + threadIdx.x;
     if (idx < 0x7fffffff) {
-        const unsigned i = (unsigned)idx, r = i / cpr;
+        const unsigned i = (unsigned)idx, r = __umulhi(i, m.mul) >> m.shift;
         row = r;
         col = (int)(i - r * cpr) * 8;
     } else {
@@ -152,7 +154,7 @@ __device__ __forceinline__ void mx_act(float x, int act, float& value, float& sl
     if (act == 1) {
         const float s = __builtin_amdgcn_rcpf(1.0f + __expf(-1.702f * x));
         value = x * s;
-        slope = s * (1.0f + 1.702f * x * (1.0f - s));
+        slope = fmaf(value, 1.702f * (1.0f - s), s);   // (x s before the other factors: nothing overflows on its way to 0 or 1)
         return;
     }
     const float z = fabsf(x) * 0.70710678118654752f, e = __expf(-0.5f * x * x);
@@ -189,7 +191,9 @@ __global__ __launch_bounds__(256) void mx_act_bwd_kernel(MxMap m, const unsigned
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         float value, slope;
-        mx_act(v[i], act, value, slope);
+        // (what rounded up to 2^128 in the checkpoint was finite: taken just below, where no 0 times infinity arises)
+        const float x = fabsf(v[i]) == INFINITY ? copysignf(3.4028234664e38f, v[i]) : v[i];
+        mx_act(x, act, value, slope);
         t[i] *= slope;
         v[i] = value;
     }
@@ -206,6 +210,10 @@ static int mx_map(MxMap& m, int64_t rows, int n, int64_t ld, const char* what) {
     m.n = n;
     m.blocks = (n + 31) / 32;
     m.ld = ld;
+    // s = ceil log2(chunks per row) and ceil(2^(31 + s) / chunks): the product is too large by under chunk 2^s, less than one step
+    m.shift = 1;
+    while ((2ll << m.shift) < 4ll * m.blocks) ++m.shift;
+    m.mul = (unsigned)(((1ull << (32 + m.shift)) + 4ull * m.blocks - 1) / (4ull * m.blocks));
     SWAT_REQUIRE(rows * (4 * (int64_t)m.blocks) <= ((int64_t)1 << 39), "%s: %lld rows of %d columns are past one launch", what, (long long)rows, n);
     return 0;
 }

@@ -10,12 +10,13 @@
 
 namespace swat {
 
-// One-dimensional work in as many workgroups as it takes: a launch holds fewer than 2^32 threads along x, the rest goes along y.
+// One-dimensional work in as many workgroups as it takes: a launch holds fewer than 2^32 threads along x, the rest goes along y.  (A
+// constant length along x: reading gridDim costs a kernel of one vector to a thread 6 %.)
 static inline dim3 mx_grid2(int64_t blocks) {
     const int64_t x = blocks < (1 << 22) ? blocks : 1 << 22;
     return dim3((unsigned)x, (unsigned)((blocks + x - 1) / x));
 }
-__device__ __forceinline__ int64_t mx_block() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
+__device__ __forceinline__ int64_t mx_block() { return ((int64_t)blockIdx.y << 22) + blockIdx.x; }
 
 // running max |x| on raw bits: NaN and infinity win over every finite value
 __device__ __forceinline__ float mx_amax(float top, float v) {

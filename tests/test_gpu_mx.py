@@ -119,6 +119,23 @@ def test_activation_slope_against_differences():
         assert ((df.double() - diff).abs() <= 2.0 ** -8 * diff.abs() + 1e-4).all()  # 2^-18 x 7, and 1e-6 of the differences
 
 
+@pytest.mark.parametrize("act", ["gelu", "quick_gelu"])
+def test_activation_of_the_largest_numbers(act):
+    """Far out the activation is x or 0 and its slope 1 or 0, also where x times a constant passes the type's end."""
+    from swat_amd import mx
+    big = torch.finfo(BF).max
+    f = torch.tensor([[big, 2.5e38, 1e38, 1e19, 1e4] + [0.0] * 27, [-big, -2.5e38, -1e38, -1e19, -1e4] + [0.0] * 27], device="cuda").to(BF)
+    g, m = mx.act_fwd(f, act)
+    assert torch.equal(g[0], f[0]) and not g[1].any()
+    for v in (big, 1e19, 1e4):   # (a block to each: small numbers next to the largest are zeros in it)
+        f = torch.tensor([[v] * 3, [-v] * 3], device="cuda").to(BF)
+        _, m = mx.act_fwd(f, act)
+        held = mx.dequantize(m)
+        df, again = mx.act_bwd(torch.ones_like(f), m, act)
+        assert torch.equal(again[0], held[0]) and not again[1].any()
+        assert (df[0] == 1).all() and not df[1].any()
+
+
 def small(got, want, mag, terms, what):
     got = got.double()
     assert torch.isfinite(got).all(), what
