@@ -60,36 +60,86 @@ __device__ __forceinline__ void mx_store4(const MxGemmArgs& p, int64_t m, int64_
         }
 }
 
-// 16 scale bytes of a row from block `first` on, blocks past the row's end as zeros.  Rows sit on any byte: where 16 bytes would reach past
-// the matrix's end the load is moved back and its bytes shifted down (the matrix has 16 bytes at least).
-__device__ __forceinline__ mx_u4 mx_scales16(const unsigned char* s, int64_t at, int64_t total) {
-    const int64_t to = at + 16 <= total ? at : total - 16;
-    mx_u4 v;
-    __builtin_memcpy(&v, s + to, 16);
-    const int sh = at - to < 16 ? (int)(at - to) : 16;
-    if (sh) {
-        unsigned w[9] = {v[0], v[1], v[2], v[3], 0u, 0u, 0u, 0u, 0u};
-        const int d = sh >> 2, b = (sh & 3) * 8;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            unsigned lo = 0u, hi = 0u;
-#pragma unroll
-            for (int j = 0; j < 5; ++j) {
-                lo = d == j ? w[i + j] : lo;
-                hi = d == j ? w[i + j + 1 < 9 ? i + j + 1 : 8] : hi;
-            }
-            v[i] = b ? lo >> b | hi << (32 - b) : lo;
-        }
+// 16 scale bytes of a row from block `first` on.  Rows sit on any byte: where 16 bytes would reach past the matrix's end (last: the row's last
+// block with 15 behind it in the matrix, may be negative) the load is moved back and its bytes shifted down (the matrix has 16 bytes at least).
+__device__ __forceinline__ mx_u4 mx_scales16(const unsigned char* row, int first, int last) {
+    const int to = first <= last ? first : last, sh = first - to;
+    uint64_t v[2];
+    __builtin_memcpy(v, row + to, 16);
+    if (__builtin_amdgcn_ballot_w64(sh != 0)) {   // (a branch of the whole wave: a divergent one in the loop over k would restructure the loop)
+        const int by = 8 * (sh & 7);
+        const uint64_t lo = sh & 8 ? v[1] : v[0], hi = sh & 8 ? 0 : v[1];
+        v[0] = lo >> by | (hi << 1) << (63 - by);
+        v[1] = hi >> by;
     }
-    return v;
+    return (mx_u4){(unsigned)v[0], (unsigned)(v[0] >> 32), (unsigned)v[1], (unsigned)(v[1] >> 32)};
 }
 
-// A workgroup computes BM x BN of C in waves of WM x WN.  Bound by the matrix cores and by the bytes a CU can load where it is large (256 x 256 in
-// 8 waves of 128 x 64: 16448 x 1024 x 4096 in 4 bits 54 us, 2.6 PFLOP/s, 8192^3 325 us, 3.4; the matrix instructions alone 29 of the
-// first's 45 us: all CUs at once run them at a lower clock than a few).  128 columns at a time: codes go through registers into one of two LDS buffers while
+// The tile of this workgroup.  Units of one XCD (workgroups b, b + 8, ..) are neighbours, 4 column tiles wide: its L2 sees few panels of
+// either operand.
+template <int BM, int BN>
+__device__ __forceinline__ void mx_tile(const MxGemmArgs& p, int64_t& m0, int64_t& n0) {
+    const int total = gridDim.x, xcd = blockIdx.x & 7, q = total >> 3, r = total & 7;
+    const int id = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (blockIdx.x >> 3);
+    const int band = id / (4 * p.tiles_m), wide = p.tiles_n - 4 * band < 4 ? p.tiles_n - 4 * band : 4;
+    const int tn = 4 * band + (id - 4 * band * p.tiles_m) % wide, tm = (id - 4 * band * p.tiles_m) / wide;
+    m0 = p.m_begin + (int64_t)tm * BM;
+    n0 = (int64_t)tn * BN;
+}
+
+// The scales of a tile's rows: 16 bytes (four tiles of k) of each at a time, on their way from memory to LDS; a thread takes one or two rows.
+// LDS: [A rows | B rows][block of the tile][tile of four].
+template <int BM, int BN, int NT>
+struct MxScales {
+    static constexpr int ROWS = BM + BN, SR = (ROWS + NT - 1) / NT;
+    mx_u4 sc[SR];
+    const unsigned char* row[SR];
+    int last[SR];
+    int next;   // group of four tiles to load next
+    int blocks;
+    __device__ __forceinline__ MxScales(const MxGemmArgs& p, int64_t m0, int64_t n0) : next(0), blocks(p.blocks) {
+#pragma unroll
+        for (int i = 0; i < SR; ++i) {
+            const int r = threadIdx.x + i * NT;
+            const bool isa = r < BM;
+            const int64_t most = isa ? p.M : p.N, at = isa ? m0 + r : n0 + (r - BM), to = at < most ? at : most - 1;   // (rows past the matrix: any scale)
+            row[i] = (isa ? p.sA : p.sB) + to * blocks;
+            const int64_t left = (most - to) * blocks - 16;
+            last[i] = left < (1 << 30) ? (int)left : 1 << 30;
+        }
+    }
+    __device__ __forceinline__ void load() {
+        const int first = 16 * next < blocks ? 16 * next : 0;
+#pragma unroll
+        for (int i = 0; i < SR; ++i) sc[i] = mx_scales16(row[i], first, last[i]);
+    }
+    __device__ __forceinline__ void put(unsigned char* to) {
+        const int have = blocks - 16 * next;   // blocks of this group inside the row; the rest gets scale byte 0 (zeros times 2^-127)
+#pragma unroll
+        for (int i = 0; i < SR; ++i) {
+            const int r = threadIdx.x + i * NT;
+            if (ROWS % NT && r >= ROWS) break;
+            unsigned w[4];
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+                const int n = have - 4 * d;
+                w[d] = sc[i][d] & (n >= 4 ? ~0u : (1u << 8 * (n > 0 ? n : 0)) - 1u);
+            }
+            // bytes [tile][block] -> [block][tile]
+            const unsigned p0 = __builtin_amdgcn_perm(w[1], w[0], 0x05010400), p1 = __builtin_amdgcn_perm(w[1], w[0], 0x07030602);
+            const unsigned q0 = __builtin_amdgcn_perm(w[3], w[2], 0x05010400), q1 = __builtin_amdgcn_perm(w[3], w[2], 0x07030602);
+            const mx_u4 t = {__builtin_amdgcn_perm(q0, p0, 0x05040100), __builtin_amdgcn_perm(q0, p0, 0x07060302),
+                             __builtin_amdgcn_perm(q1, p1, 0x05040100), __builtin_amdgcn_perm(q1, p1, 0x07060302)};
+            *reinterpret_cast<mx_u4*>(to + r * 16) = t;
+        }
+        ++next;
+    }
+};
+
+// A workgroup computes BM x BN of C in waves of WM x WN, 128 columns at a time: codes go through registers into one of two LDS buffers while
 // the matrix cores work on the other, loads two tiles ahead.  A row's scales come 16 bytes (four tiles) at a time, are transposed to
 // [block of the tile][tile] and kept in LDS, so that one 4-byte read gives a lane the scales of its row and block for four tiles, which
-// the instruction picks by byte.
+// the instruction picks by byte.  16384 x 1024 x 4096 in 256 x 256 (8 waves of 128 x 64): 8 by 8 bits 70 us, 8 by 4 61 (2.2 PFLOP/s).
 template <int AB, int BB, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, 2) void mx_gemm_kernel(MxGemmArgs p) {
     constexpr int NT = (BM / WM) * (BN / WN) * 64, FM = WM / 16, FN = WN / 16;
@@ -98,18 +148,11 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, 2) void mx_gemm_kernel(
     constexpr int BUF = BM * RA + BN * RB, ROWS = BM + BN;
     static_assert(CA * NT == BM * CRA && CB * NT == BN * CRB && RSA % 16 == 0 && RSB % 16 == 0 && ROWS <= 2 * NT, "whole chunks");
     __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * BUF + 2 * ROWS * 16];
-    unsigned char* const ssc = smem + 2 * BUF;   // scales: [2][A rows | B rows][block of the tile][tile of four]
+    unsigned char* const ssc = smem + 2 * BUF;   // two groups of scales
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int r16 = lane & 15, g = lane >> 4, wr = wave / (BN / WN), wc = wave % (BN / WN);
-    // units of one XCD (workgroups b, b + 8, ..) are neighbours, 4 column tiles wide: its L2 sees few panels of either operand
-    int id;
-    {
-        const int total = gridDim.x, xcd = blockIdx.x & 7, q = total >> 3, r = total & 7;
-        id = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (blockIdx.x >> 3);
-    }
-    const int band = id / (4 * p.tiles_m), wide = p.tiles_n - 4 * band < 4 ? p.tiles_n - 4 * band : 4;
-    const int tn = 4 * band + (id - 4 * band * p.tiles_m) % wide, tm = (id - 4 * band * p.tiles_m) / wide;
-    const int64_t m0 = p.m_begin + (int64_t)tm * BM, n0 = (int64_t)tn * BN;
+    int64_t m0, n0;
+    mx_tile<BM, BN>(p, m0, n0);
     const int rowA = p.blocks * 4 * AB, rowB = p.blocks * 4 * BB;   // bytes of a packed row
     const int nk = (p.blocks + 3) / 4;
 
@@ -147,40 +190,7 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, 2) void mx_gemm_kernel(
 #pragma unroll
         for (int i = 0; i < CB; ++i) *reinterpret_cast<mx_u4*>(wb + buf * BUF + i * RSB * RB) = st.b[i];
     };
-    // scales: a thread takes one or two rows of the tile
-    constexpr int SR = (ROWS + NT - 1) / NT;
-    mx_u4 sc[SR];
-    int s_next = 0;   // next group of four tiles to load
-    auto load_scales = [&]() {
-#pragma unroll
-        for (int i = 0; i < SR; ++i) {
-            const int r = tid + i * NT;
-            const bool isa = r < BM;
-            int64_t row = isa ? m0 + r : n0 + (r - BM);
-            const int64_t most = isa ? p.M : p.N;
-            row = row < most ? row : most - 1;   // (rows past the matrix: any scale, their codes are zeros)
-            const int first = 16 * s_next < p.blocks ? 16 * s_next : 0;
-            sc[i] = mx_scales16(isa ? p.sA : p.sB, row * p.blocks + first, most * p.blocks);
-        }
-    };
-    auto put_scales = [&](int buf) {
-        const int have = p.blocks - 16 * s_next;   // blocks of this group inside the row; the rest gets scale byte 0 (zeros times 2^-127)
-#pragma unroll
-        for (int i = 0; i < SR; ++i) {
-            const int r = tid + i * NT;
-            if (ROWS % NT && r >= ROWS) break;
-            unsigned w[4];
-#pragma unroll
-            for (int d = 0; d < 4; ++d) w[d] = have >= 4 * d + 4 ? sc[i][d] : have <= 4 * d ? 0u : sc[i][d] & ((1u << 8 * (have - 4 * d)) - 1u);
-            // bytes [tile][block] -> [block][tile]
-            const unsigned p0 = __builtin_amdgcn_perm(w[1], w[0], 0x05010400), p1 = __builtin_amdgcn_perm(w[1], w[0], 0x07030602);
-            const unsigned q0 = __builtin_amdgcn_perm(w[3], w[2], 0x05010400), q1 = __builtin_amdgcn_perm(w[3], w[2], 0x07030602);
-            const mx_u4 t = {__builtin_amdgcn_perm(q0, p0, 0x05040100), __builtin_amdgcn_perm(q0, p0, 0x07060302),
-                             __builtin_amdgcn_perm(q1, p1, 0x05040100), __builtin_amdgcn_perm(q1, p1, 0x07060302)};
-            *reinterpret_cast<mx_u4*>(ssc + (buf * ROWS + r) * 16) = t;
-        }
-        ++s_next;
-    };
+    MxScales<BM, BN, NT> sc(p, m0, n0);
     auto bar = [&]() {
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
@@ -227,11 +237,11 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, 2) void mx_gemm_kernel(
         }
     };
 
-    load_scales();
+    sc.load();
     load(st0);
     if constexpr (DEEP) load(st1);
-    put_scales(0);
-    load_scales();
+    sc.put(ssc);
+    sc.load();
     put(st0, 0);
     load(st0);
     bar();
@@ -250,8 +260,8 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, 2) void mx_gemm_kernel(
         if (++t >= nk) break;
         put(st1, 1);
         load(st1);
-        put_scales(sbuf ^ 1);   // (read last two tiles ago)
-        load_scales();
+        sc.put(ssc + (sbuf ^ 1) * ROWS * 16);   // (read last two tiles ago)
+        sc.load();
         multiply(0, std::integral_constant<int, 2>{});
         bar();
         if (++t >= nk) break;
@@ -261,6 +271,152 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, 2) void mx_gemm_kernel(
         bar();
         if (++t >= nk) break;
     }
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) mx_store4(p, m0 + WM * wr + 16 * i + r16, n0 + WN * wc + 16 * j + 4 * g, acc[i][j]);
+}
+
+// The same for 4 by 4 bits in tiles of 128 and more, whose codes come straight into LDS, three tiles ahead, in a ring of four buffers: the loads
+// cost no registers, so that there is room to read the next tile's B and half of its A while this tile's second half multiplies, and they
+// may take the time of two tiles.  16448 x 1024 x 4096: 54.5 -> 47.7 us, 8192^3 323 -> 273 (4.0 PFLOP/s; in 128 x 128 405 -> 386).  Bound by
+// the matrix cores and LDS in turn: without loads and LDS reads 16384 x 1024 x 4096 takes 33 of its 46 us, of which 16 are what the
+// matrix instructions take from registers with every CU on them (8.7 PFLOP/s).
+// What a load past an edge leaves in LDS (the next row's codes, zeros or older codes) is multiplied by block scales of zero bytes, 2^-127 on
+// both sides, or belongs to rows that are not stored: an e2m1 code is always finite.
+template <int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, 2) void mx_ring_kernel(MxGemmArgs p) {
+    constexpr int NW = (BM / WM) * (BN / WN), NT = 64 * NW, FM = WM / 16, FN = WN / 16;
+    constexpr int ROWS = BM + BN, BUF = 64 * ROWS, LOADS = ROWS / NW / 16;   // a tile: 64 bytes of each row; loads to a wave
+    static_assert(BM % (16 * NW) == 0 && BN % (16 * NW) == 0 && 2 * LOADS < 16, "whole loads; their count fits the wait");
+    __shared__ __attribute__((aligned(1024))) unsigned char ring0[BUF], ring1[BUF], ring2[BUF], ring3[BUF];
+    __shared__ __attribute__((aligned(1024))) unsigned char ssc[2 * ROWS * 16];   // two groups of scales
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r16 = lane & 15, g = lane >> 4, wr = wave / (BN / WN), wc = wave % (BN / WN);
+    int64_t m0, n0;
+    mx_tile<BM, BN>(p, m0, n0);
+    const int row = p.blocks * 16;   // bytes of a packed row
+    const int nk = (p.blocks + 3) / 4;
+
+    // codes: buffer descriptors that start at the tile's rows and end with the matrix, advanced along k
+    const int rowsA = p.M - m0 < BM ? (int)(p.M - m0) : BM, rowsB = p.N - n0 < BN ? (int)(p.N - n0) : BN;
+    const unsigned char *ga = p.A + m0 * row, *gb = p.B + n0 * row;
+    int left = row;   // bytes of a row still to load (<= 0: past the last tile)
+    // a load fills 16 rows in LDS, lane l bytes 16 l .. of them: the permutation is on what a lane loads
+    const int lr = lane >> 2, lc = (lane & 3) ^ ((lane >> 4) & 3);
+    const unsigned oa = (unsigned)((wave * (BM / NW) + lr) * row + lc * 16), ob = (unsigned)((wave * (BN / NW) + lr) * row + lc * 16);
+    auto ring = [&](auto n) -> unsigned char* {
+        constexpr int R = decltype(n)::value & 3;
+        if constexpr (R == 0) return ring0;
+        else if constexpr (R == 1) return ring1;
+        else if constexpr (R == 2) return ring2;
+        else return ring3;
+    };
+    auto load = [&](auto n) {
+        unsigned char* to = ring(n);
+        const __amdgpu_buffer_rsrc_t da = __builtin_amdgcn_make_buffer_rsrc((void*)ga, 0, left > 0 ? (rowsA - 1) * row + left : 0, 0x20000);
+        const __amdgpu_buffer_rsrc_t db = __builtin_amdgcn_make_buffer_rsrc((void*)gb, 0, left > 0 ? (rowsB - 1) * row + left : 0, 0x20000);
+#pragma unroll
+        for (int i = 0; i < BM / NW / 16; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(da, (__attribute__((address_space(3))) void*)(to + (wave * (BM / NW) + 16 * i) * 64), 16, oa + (unsigned)(16 * i * row), 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < BN / NW / 16; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(db, (__attribute__((address_space(3))) void*)(to + BM * 64 + (wave * (BN / NW) + 16 * i) * 64), 16, ob + (unsigned)(16 * i * row), 0, 0, 0);
+        ga += 64;
+        gb += 64;
+        left -= 64;
+    };
+    MxScales<BM, BN, NT> sc(p, m0, n0);
+    auto bar = [&]() {   // (all but the newest two tiles' loads)
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0x70 | (2 * LOADS));
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+
+    f32x4_t acc[FM][FN];
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+    int sa[FM], sb[FN];
+    auto read_scales = [&](int buf) {
+        const unsigned char* q = ssc + buf * ROWS * 16 + 4 * g;
+#pragma unroll
+        for (int i = 0; i < FM; ++i) sa[i] = *reinterpret_cast<const int*>(q + (WM * wr + 16 * i + r16) * 16);
+#pragma unroll
+        for (int j = 0; j < FN; ++j) sb[j] = *reinterpret_cast<const int*>(q + (BM + WN * wc + 16 * j + r16) * 16);
+    };
+    int fa0 = WM * wr * 64 + mx_lds_off<4>(r16, g), fb0 = (BM + WN * wc) * 64 + mx_lds_off<4>(r16, g);
+    mx_u4 qa[FM], qb[2][FN];
+    auto read_a = [&](auto n, auto half) {
+        constexpr int I0 = decltype(half)::value * (FM / 2);
+        const unsigned char* q = ring(n) + fa0;
+#pragma unroll
+        for (int i = I0; i < I0 + FM / 2; ++i) qa[i] = *reinterpret_cast<const mx_u4*>(q + 16 * i * 64);
+    };
+    auto read_b = [&](auto n) {
+        const unsigned char* q = ring(n) + fb0;
+#pragma unroll
+        for (int j = 0; j < FN; ++j) qb[decltype(n)::value & 1][j] = *reinterpret_cast<const mx_u4*>(q + 16 * j * 64);
+    };
+    auto four = [](mx_u4 v) { return (mx_v8i){(int)v[0], (int)v[1], (int)v[2], (int)v[3], 0, 0, 0, 0}; };
+    auto half_tile = [&](auto n, auto half) {
+        constexpr int I0 = decltype(half)::value * (FM / 2), S = decltype(n)::value;
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int i = I0; i < I0 + FM / 2; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) acc[i][j] = mx_mfma<4, 4, S>(four(qb[S & 1][j]), four(qa[i]), acc[i][j], sb[j], sa[i]);
+        __builtin_amdgcn_s_setprio(0);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    constexpr std::integral_constant<int, 0> H0{};
+    constexpr std::integral_constant<int, 1> H1{};
+    auto step = [&](auto n, int sbuf) {
+        constexpr int S = decltype(n)::value;
+        constexpr std::integral_constant<int, (S + 1) & 3> N1{};
+        constexpr std::integral_constant<int, (S + 3) & 3> N3{};
+        asm volatile("" : "+v"(fa0), "+v"(fb0));   // (sums of these and a buffer's address are made anew, not kept in registers)
+        if constexpr (S == 0) read_scales(sbuf);
+        read_a(n, H1);
+        __builtin_amdgcn_sched_barrier(0);
+        load(N3);
+        if constexpr (S == 2) {
+            sc.put(ssc + (sbuf ^ 1) * ROWS * 16);   // (read last two tiles ago)
+            sc.load();
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        half_tile(n, H0);
+        bar();
+        read_b(N1);
+        read_a(N1, H0);
+        __builtin_amdgcn_sched_barrier(0);
+        half_tile(n, H1);
+    };
+    constexpr std::integral_constant<int, 0> T0{};
+    constexpr std::integral_constant<int, 1> T1{};
+    constexpr std::integral_constant<int, 2> T2{};
+    constexpr std::integral_constant<int, 3> T3{};
+    sc.load();
+    load(T0);
+    load(T1);
+    load(T2);
+    sc.put(ssc);
+    sc.load();
+    bar();
+    read_b(T0);
+    read_a(T0, H0);
+    int t = 0;
+    for (int sbuf = 0;; sbuf ^= 1) {   // (a tile past the last one multiplies by scales of zero)
+        step(T0, sbuf);
+        step(T1, sbuf);
+        if ((t += 2) >= nk) break;
+        step(T2, sbuf);
+        step(T3, sbuf);
+        if ((t += 2) >= nk) break;
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (no load may reach LDS after the workgroup has left it)
 #pragma unroll
     for (int i = 0; i < FM; ++i)
 #pragma unroll
@@ -373,17 +529,18 @@ static bool mx_tiles(MxGemmArgs p, int64_t rows, hipStream_t s) {
     p.tiles_n = (int)((p.N + BN - 1) / BN);
     const int64_t grid = (int64_t)p.tiles_m * p.tiles_n;
     if (grid >= 1 << 23) return false;
-    mx_gemm_kernel<AB, BB, BM, BN, WM, WN><<<(unsigned)grid, (BM / WM) * (BN / WN) * 64, 0, s>>>(p);
+    if constexpr (AB + BB == 8 && BM >= 128) mx_ring_kernel<BM, BN, WM, WN><<<(unsigned)grid, (BM / WM) * (BN / WN) * 64, 0, s>>>(p);
+    else mx_gemm_kernel<AB, BB, BM, BN, WM, WN><<<(unsigned)grid, (BM / WM) * (BN / WN) * 64, 0, s>>>(p);
     return true;
 }
 
-// Which tile, by the sum of what was measured (us, 4 by 4 bits; an 8-bit operand adds 28 %): a 128-column step takes a CU 0.8 with five
-// 64 x 64 workgroups on it (0.25 with one), 0.78 with two of 128 x 128 (0.45 with one), 1.2 with one of 256 x 256; a round of workgroups
-// 2.5, 3.5, 7 more (the last is alone on its CU while it stores).  Up to 64 rows past whole tiles may go to mx_rows (5) instead of a round of
-// their own.  Few rows and columns: mx_rows.
-//   4 x 4 bits, 64 x 64 / 128 x 128 / 256 x 256: 1600 x 768 x 768 5.9 / 7.5 / 15.8; 8239 x 2048 x 1000 35 / 28.1 / 37.8 (25.9 with the last rows
-//   apart); 16448 x 1024 x 4096 110 / 68 / 87 (53.9); 8192^3 795 / 416 / 325.   64 rows, 1024 x 4096 5.7 in mx_rows, 11.1 in 64 x 64;
-//   64 rows, 65536 x 512 20 and 8.2
+// Which tile, by the sum of what was measured (us): a 128-column step takes a CU, 4 by 4 bits, 0.8 with five 64 x 64 workgroups on it (0.25
+// with one), 0.73 with two of 128 x 128 (0.4 with one), 0.97 with one of 256 x 256; with 8-bit operands 0.8, 0.78 (0.45), 1.2 and 28 % more
+// for each of them; a round of workgroups 2.5, 3.5, 7 more (the last is alone on its CU while it stores).  Up to 64 rows past whole tiles
+// may go to mx_rows (5) instead of a round of their own.  Few rows and columns: mx_rows.
+//   4 x 4 bits, 64 x 64 / 128 x 128 / 256 x 256: 1600 x 768 x 768 10.4 / 10.1 / 17.1; 4096 x 1024 x 1024 11.6 / 10.1 / 16.9; 2048 x 4096 x 4096 62 /
+//   31.9 / 36.2; 8239 x 2048 x 1000 36 / 27.9 / 25.6; 16448 x 1024 x 4096 108 / 66 / 47.7; 8192^3 797 / 386 / 273.   64 rows, 1024 x 4096 5.7 in
+//   mx_rows, 11.1 in 64 x 64; 64 rows, 65536 x 512 20 and 8.2
 struct MxGemmPlan {
     int size;        // 0: mx_rows, 1: 64 x 64, 2: 128 x 128, 3: 256 x 256
     int64_t rows;    // those of the tile kernel; what is behind goes to mx_rows
@@ -392,7 +549,9 @@ static MxGemmPlan mx_plan(int64_t M, int64_t N, int blocks, int ab, int bb) {
     const int64_t cols16 = (N + 15) / 16;
     // (fewer than 16 scale bytes in an operand: the tile kernels load them by 16)
     if ((M <= 64 && cols16 <= 512) || M * blocks < 16 || N * blocks < 16) return {0, 0};
-    static const double full[4] = {0, 0.8, 0.78, 1.2}, alone[4] = {0, 0.25, 0.45, 1.2}, round[4] = {0, 2.5, 3.5, 7.0};
+    static const double full4[4] = {0, 0.8, 0.73, 0.97}, alone4[4] = {0, 0.25, 0.4, 0.97}, full8[4] = {0, 0.8, 0.78, 1.2}, alone8[4] = {0, 0.25, 0.45, 1.2};
+    static const double round[4] = {0, 2.5, 3.5, 7.0};
+    const double *full = ab + bb == 8 ? full4 : full8, *alone = ab + bb == 8 ? alone4 : alone8;
     static const int slots[4] = {0, 5, 2, 1};
     const double f = 1.0 + 0.07 * (ab + bb - 8), steps = (blocks + 3) / 4;
     MxGemmPlan best = {};
