@@ -494,7 +494,8 @@ int swat_preprocess_batch(const void* pixels_u8, const int64_t* offsets, const i
  *     rows.  x and y share x_dtype; x, h: row strides in elements, d at least; y, z: contiguous.  stats fp32 [4][rows] (may be null):
  *     mean and 1 / deviation of Norm_post, of Norm_pre — what the backward call reads; rows of a norm that is not there stay as they
  *     were.  z8_codes / z8_scales (both or neither): z once more, packed to 8 bits as swat_mx_quantize would pack the z written beside
- *     it (z may then be null).  1 <= d <= 8192.  Rows that do not sit on 16 (bf16: 8) bytes or d % 4 != 0 take a slower path. */
+ *     it (z may then be null), z8_codes on 4 bytes.  1 <= d <= 8192; rows start on any element; 2^25 gates at most unless every row has its
+ *     own (a row of gates: 2^25 / (4 ceil(d / 256))). */
 int swat_residual_norm_fwd(const void* x, int64_t x_stride, int x_dtype, const void* h, int64_t h_stride, int h_dtype,
                            const float* post_w, const float* post_b, const float* gate, int64_t groups, int gate_channels,
                            const float* scale, const float* pre_w, const float* pre_b, float alpha, int rms, float eps,
@@ -502,7 +503,9 @@ int swat_residual_norm_fwd(const void* x, int64_t x_stride, int x_dtype, const v
                            swat_stream_t stream);
 /*     its backward: dy (may be null: zero; x_dtype) and dz (z_dtype; null without pre_w) -> dx (x_dtype), dh (h_dtype) and the
  *     gradients of everything that was given (a pointer may be null to leave one out; dgate goes with gate).  y: the forward's
- *     output.  All sums in a fixed order (deterministic); gradients are written, not accumulated.  dh is zero where m is zero.
+ *     output.  All sums in a fixed order (deterministic); gradients are written, not accumulated.  dh is zero where m is zero, and so is
+ *     what such an element gives the norm's weights; a gate's gradient leaves out channels whose scale is zero, a scale's rows whose
+ *     gate is zero (a zero gate's own gradient is what its branch holds).
  *     workspace: swat_residual_norm_bwd_workspace_bytes(rows, d, groups (0: no gate), gate_channels) bytes on 16 bytes. */
 int64_t swat_residual_norm_bwd_workspace_bytes(int rows, int d, int64_t groups, int gate_channels);
 int swat_residual_norm_bwd(const void* dy, int64_t dy_stride, const void* dz, int64_t dz_stride, int z_dtype, const void* h,
@@ -516,7 +519,8 @@ int swat_residual_norm_bwd(const void* dy, int64_t dy_stride, const void* dz, in
  *     or e2m1 (4 bits, up to 6).  E = the smallest with max |x| 2^-E within the format, -110 at least (so every held value is a
  *     normal bfloat16); elements are x 2^-E rounded to nearest even.  A block that held a NaN or an infinity is NaN as a whole
  *     (byte 255).  codes uint8 [rows, ceil(n / 32) * 32 * bits / 8] (4 bits: the even column in the low half; the columns behind n
- *     are zeros), on 16 bytes; scales uint8 [rows, ceil(n / 32)]. */
+ *     are zeros), on 16 bytes; scales uint8 [rows, ceil(n / 32)].  1 <= n <= 2^24; values start on any element.  (In the top binade a
+ *     number can round up to 2^128, which fp32 and bf16 hold as infinity.) */
 int swat_mx_quantize(const void* x, int64_t x_stride, int x_dtype, int bits, void* codes, void* scales, int64_t rows, int n,
                      swat_stream_t stream);
 int swat_mx_dequantize(const void* codes, const void* scales, int bits, void* out, int out_dtype, int64_t rows, int n,
@@ -529,14 +533,16 @@ int swat_mx_act_bwd(const void* dg_bf16, int64_t dg_stride, const void* codes, c
                     int64_t rows, int n, swat_stream_t stream);
 /* Weight gradient of a linear layer whose input was kept as an 8-bit checkpoint: dW [n_out, n_in] = dY^T X8 (fp32, written),
  *     dbias [n_out] = column sums of dY (may be null).  dY bf16 [rows, n_out] with a row stride.  Unpacking is exact, accumulation
- *     fp32, the order of the sums fixed.  workspace: swat_mx_linear_wgrad_workspace_bytes(...) bytes on 16 bytes (0: null will do). */
+ *     fp32, the order of the sums fixed.  dY starts on any element, its row stride is 2^23 at most; n_in <= 2^24, n_out n_in < 2^34; dW sits
+ *     on 16 bytes.  workspace: swat_mx_linear_wgrad_workspace_bytes(...) bytes on 16 bytes (0: null will do). */
 int64_t swat_mx_linear_wgrad_workspace_bytes(int64_t rows, int n_out, int n_in);
 int swat_mx_linear_wgrad(const void* dY_bf16, int64_t dy_stride, const void* x_codes, const void* x_scales, float* dW, float* dbias,
                          int64_t rows, int n_out, int n_in, void* workspace, int64_t workspace_bytes, swat_stream_t stream);
 /* C [M, N] = A B^T (+ bias fp32 [N]) of packed A [M, K], B [N, K], 4 or 8 bits each, on the scaled matrix instructions (nothing is
  *     unpacked; fp32 accumulation).  c_dtype bf16, or fp32 where both operands have 4 bits: with an 8-bit operand the instruction drops
  *     what lies more than 13 binary places below the largest of eight neighbouring columns' products, far under the operands' own
- *     rounding (2^-4) and bf16's (2^-8), but not under fp32's.  Codes, bias and C sit on 16 bytes. */
+ *     rounding (2^-4) and bf16's (2^-8), but not under fp32's.  Codes, bias and C sit on 16 bytes; K <= 2^22, M and N <= 2^30 and
+ *     fewer than 2^23 tiles (refused otherwise). */
 int swat_mx_matmul(const void* a_codes, const void* a_scales, int a_bits, const void* b_codes, const void* b_scales, int b_bits,
                    const float* bias, void* c, int c_dtype, int64_t M, int64_t N, int K, swat_stream_t stream);
 

@@ -30,15 +30,18 @@ struct MxWgradArgs {
 
 // A workgroup computes BN x BK of dW over its share of the rows; waves of WN x WK.  64 rows at a time: both operands go through
 // registers into one of two LDS buffers ([64 rows][columns], 16-byte chunks permuted so that neither the writes nor the transposing
-// reads meet in a bank) while the matrix cores work on the other; the global loads run a whole tile ahead.
-template <int BN, int BK, int WN, int WK>
-__global__ __launch_bounds__((BN / WN) * (BK / WK) * 64, 2) void mx_wgrad_kernel(MxWgradArgs p) {
+// reads meet in a bank) while the matrix cores work on the other; the global loads run a whole tile ahead.  GROUPS of such waves share the
+// rows where there are few tiles of dW (one workgroup to a CU waits for a tile's latency: 0.43 us, two 0.27 each); their sums meet in LDS,
+// the first group's first.
+template <int BN, int BK, int WN, int WK, int GROUPS>
+__global__ __launch_bounds__((BN / WN) * (BK / WK) * 64 * GROUPS, 2) void mx_wgrad_kernel(MxWgradArgs p) {
     constexpr int NT = (BN / WN) * (BK / WK) * 64, FN = WN / 16, FK = WK / 16;
     constexpr int YB = 64 * BN * 2, XB = 64 * BK * 2;
     constexpr int YC = 64 * BN / 8 / NT, XC = 64 * BK / 16 / NT;   // chunks to a thread: 8 columns of dY, 16 of X
     static_assert(YC * NT * 8 == 64 * BN && XC * NT * 16 == 64 * BK, "whole chunks");
-    __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * (YB + XB)];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    __shared__ __attribute__((aligned(1024))) unsigned char shared[GROUPS * 2 * (YB + XB)];
+    const int group = GROUPS > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / NT) : 0, tid = threadIdx.x - group * NT, lane = tid & 63, wave = tid >> 6;
+    unsigned char* const smem = shared + group * 2 * (YB + XB);
     const int r16 = lane & 15, g = lane >> 4, wr = wave / (BK / WK), wc = wave % (BK / WK);
     // units of one XCD (workgroups b, b + 8, ..) are neighbours: the same rows, 4 k tiles wide, so that its L2 sees few panels of dY and X
     int id;
@@ -50,8 +53,10 @@ __global__ __launch_bounds__((BN / WN) * (BK / WK) * 64, 2) void mx_wgrad_kernel
     const int band = in / (4 * p.tiles_n), wide = p.tiles_k - 4 * band < 4 ? p.tiles_k - 4 * band : 4;
     const int tk = 4 * band + (in - 4 * band * p.tiles_n) % wide, tn = (in - 4 * band * p.tiles_n) / wide;
     const int n0 = tn * BN, k0 = tk * BK;
-    const int64_t t0 = (int64_t)split * p.tiles_per_split, all = (p.rows + 63) / 64;
-    const int nt = (int)(t0 + p.tiles_per_split < all ? p.tiles_per_split : all > t0 ? all - t0 : 0);
+    // this split's tiles, the same number to a group (those behind the last row, and behind the split's, are empty)
+    const int64_t s0 = (int64_t)split * p.tiles_per_split, all = (p.rows + 63) / 64;
+    const int whole = (int)(s0 + p.tiles_per_split < all ? p.tiles_per_split : all > s0 ? all - s0 : 0), nt = (whole + GROUPS - 1) / GROUPS;
+    const int64_t t0 = s0 + group * nt, end_tile = t0 + nt < s0 + whole ? t0 + nt : s0 + whole, end = end_tile * 64 < p.rows ? end_tile * 64 : p.rows;
 
     // Global loads go through buffer descriptors that end with the matrix: rows past the last one read as zeros, columns past the edge get
     // an offset past the end.  dY may sit on any 2 bytes; the range check is by whole dwords, so with an odd n the matrix's very last
@@ -75,10 +80,11 @@ __global__ __launch_bounds__((BN / WN) * (BK / WK) * 64, 2) void mx_wgrad_kernel
     const unsigned os = xcol < xld ? (unsigned)(xrow * p.blocks + (xcol >> 5)) : OUT;
     unsigned char *const wy = smem + stp_off<BN>(yrow, ycol - n0), *const wx = smem + 2 * YB + stp_off<BK>(xrow, xcol - k0);
     auto load = [&](Stage& st, int t) {
-        const int64_t m0 = (t0 + t) * 64 < p.rows ? (t0 + t) * 64 : p.rows, left = p.rows - m0;
+        const int64_t m0 = (t0 + t) * 64 < end ? (t0 + t) * 64 : end, left = end - m0;
         const int rows = left < 64 ? (int)left : 64;   // (a tile with rows behind it: one element more, its last dword may reach into the next)
+        const bool behind = p.rows - m0 > 64;
         const __amdgpu_buffer_rsrc_t by = __builtin_amdgcn_make_buffer_rsrc((void*)(p.dY + m0 * p.ld), 0,
-                                                                             left > 64 ? 128 * (int)p.ld + 2 : rows ? 2 * ((rows - 1) * (int)p.ld + p.n) : 0, 0x20000);
+                                                                             !rows ? 0 : behind ? 128 * (int)p.ld + 2 : 2 * ((rows - 1) * (int)p.ld + p.n), 0x20000);
         const __amdgpu_buffer_rsrc_t bx = __builtin_amdgcn_make_buffer_rsrc((void*)(p.X + m0 * xld), 0, rows * xld, 0x20000);
         const __amdgpu_buffer_rsrc_t bs = __builtin_amdgcn_make_buffer_rsrc((void*)(p.S + m0 * p.blocks), 0, rows * p.blocks, 0x20000);
 #pragma unroll
@@ -196,20 +202,52 @@ __global__ __launch_bounds__((BN / WN) * (BK / WK) * 64, 2) void mx_wgrad_kernel
         multiply(f1);
     }
     bar();
-    const bool odd_end = (p.n & 1) && nt > 0 && t0 + nt == all;   // (see the loads)
+    const bool odd_end = (p.n & 1) && end == p.rows && t0 * 64 < end;   // (see the loads)
     if (sums) {   // the threads that share 8 columns meet in LDS (tiles are done with it), rows of threads added in order
-        float* cp = reinterpret_cast<float*>(smem);
+        float* cp = reinterpret_cast<float*>(shared);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) cp[(tid / (BN / 8)) * BN + 8 * (tid % (BN / 8)) + e] = cs[e];
+        for (int e = 0; e < 8; ++e) cp[((int)threadIdx.x / (BN / 8)) * BN + 8 * (tid % (BN / 8)) + e] = cs[e];
         bar();
-        for (int c = tid; c < BN; c += NT)
+        for (int c = threadIdx.x; c < BN; c += GROUPS * NT)
             if (n0 + c < p.n) {
                 float t = 0.f;
 #pragma unroll
-                for (int r = 0; r < NT / (BN / 8); ++r) t += cp[r * BN + c];
-                if (odd_end && n0 + c == p.n - 1) t += bf2f(p.dY[(p.rows - 1) * p.ld + n0 + c]);
+                for (int r = 0; r < GROUPS * NT / (BN / 8); ++r) t += cp[r * BN + c];
+                if ((p.n & 1) && whole > 0 && s0 + whole == all && n0 + c == p.n - 1) t += bf2f(p.dY[(p.rows - 1) * p.ld + n0 + c]);
                 p.db[(int64_t)split * p.n + n0 + c] = t;
             }
+    }
+    if (odd_end) {
+#pragma unroll
+        for (int i = 0; i < FN; ++i) {
+            if (n0 + WN * wr + 16 * i + r16 != p.n - 1) continue;
+            const float y = bf2f(p.dY[(p.rows - 1) * p.ld + p.n - 1]);
+#pragma unroll
+            for (int j = 0; j < FK; ++j) {
+                const int k = k0 + WK * wc + 16 * j + 4 * g;
+                if (k >= xld) continue;
+                float x[4];
+                mx_from_e4m3x4(*reinterpret_cast<const unsigned*>(p.X + (p.rows - 1) * xld + k), mx_scale(p.S[(p.rows - 1) * p.blocks + (k >> 5)]), x);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(y, x[e], acc[i][j][e]);
+            }
+        }
+    }
+    if constexpr (GROUPS > 1) {
+        static_assert(GROUPS == 2 && FN * FK * NT * 16 <= 4 * (YB + XB), "one sum in LDS");
+        if (sums) bar();
+        f32x4_t* const other = reinterpret_cast<f32x4_t*>(shared);
+        if (group)
+#pragma unroll
+            for (int i = 0; i < FN; ++i)
+#pragma unroll
+                for (int j = 0; j < FK; ++j) other[(i * FK + j) * NT + tid] = acc[i][j];
+        bar();
+        if (group) return;
+#pragma unroll
+        for (int i = 0; i < FN; ++i)
+#pragma unroll
+            for (int j = 0; j < FK; ++j) acc[i][j] += other[(i * FK + j) * NT + tid];
     }
     float* dW = p.dW + (int64_t)split * p.n * p.k;
 #pragma unroll
@@ -219,13 +257,6 @@ __global__ __launch_bounds__((BN / WN) * (BK / WK) * 64, 2) void mx_wgrad_kernel
 #pragma unroll
         for (int j = 0; j < FK; ++j) {
             const int k = k0 + WK * wc + 16 * j + 4 * g;
-            if (odd_end && n == p.n - 1 && k < xld) {
-                const float y = bf2f(p.dY[(p.rows - 1) * p.ld + n]);
-                float x[4];
-                mx_from_e4m3x4(*reinterpret_cast<const unsigned*>(p.X + (p.rows - 1) * xld + k), mx_scale(p.S[(p.rows - 1) * p.blocks + (k >> 5)]), x);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(y, x[e], acc[i][j][e]);
-            }
             float* out = dW + (int64_t)n * p.k + k;
             if (p.k % 4 == 0) {
                 if (k < p.k) *reinterpret_cast<float4*>(out) = make_float4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]);
@@ -266,27 +297,31 @@ __global__ __launch_bounds__(256) void mx_wgrad_join_kernel(const float* pw, con
 }
 
 struct MxWgradPlan {
-    int big, tiles_n, tiles_k, splits, per;
+    int form;   // 0: 64 x 64, 1: 128 x 256, 2: 64 x 64 in two groups
+    int tiles_n, tiles_k, splits, per;
 };
-// 128 x 256 tiles (8 waves, one workgroup to a CU) or 64 x 64 (4 waves, up to four), and into how many parts the rows are split, by the
-// sum of what was measured (us): a 64-row tile takes 1.02 in the first form; in the second 0.43 alone on its CU and 0.27 for each of
-// several; 6.5 / 3 to start and to store; a join 2.5 and its planes' bytes at 4.5 TB/s.  At 16448 rows, 4096 x 1024: 150 in the first
-// form with 2 parts (259 with 1, 157 with 4), 240 in the second; at 1600 rows, 768 x 768: 13.7 in the second (1 part), 21.4 in the first.
+// 128 x 256 tiles (8 waves, one workgroup to a CU), 64 x 64 (4 waves, up to four) or, while those are one to a CU, 64 x 64 in two groups of
+// waves, and into how many parts the rows are split, by the sum of what was measured (us): a 64-row tile takes 1.02 in the first form, 0.43
+// in the second alone on its CU and 0.27 for each of several; 6.5 / 3 to start and to store; a join of parts 4 and its planes' bytes at 4.5
+// TB/s.  At 16448 rows, 4096 x 1024: 150 in the first form with 2 parts (259 with 1, 157 with 4), 240 in the second; at 1600 rows,
+// 768 x 768: 12.5 in two groups, 15 in one (2, 3, 4 parts: 15.3, 14.5, 16.9), 21.4 in the first; 6304 rows: 47.8 in one part, 35, 27.4, 28.4 in more.
 static MxWgradPlan mx_wgrad_plan(int64_t rows, int n, int k) {
     const int64_t all = (rows + 63) / 64;
     MxWgradPlan best = {};
     double cost = -1;
-    for (int big = 0; big < 2; ++big) {
+    for (int form = 0; form < 3; ++form) {
+        const bool big = form == 1;
         const int bn = big ? 128 : 64, bk = big ? 256 : 64;
-        MxWgradPlan p = {big, (n + bn - 1) / bn, (k + bk - 1) / bk, 1, 1};
+        MxWgradPlan p = {form, (n + bn - 1) / bn, (k + bk - 1) / bk, 1, 1};
         for (int s = 1; s <= 16 && (s == 1 || s <= all); ++s) {
             p.per = all > 0 ? (int)((all + s - 1) / s) : 1;
             p.splits = all > 0 ? (int)((all + p.per - 1) / p.per) : 1;
             if (p.splits != s) continue;
             const double units = (double)p.tiles_n * p.tiles_k * s, rounds = ceil(units / (big ? 256 : 1024));
+            if (form == 2 && units > 256) continue;
             const double at_once = units > 1024 ? 4 : ceil(units / 256);
-            const double tile = big ? 1.02 : at_once < 2 ? 0.43 : 0.27 * at_once;
-            const double c = (big ? 6.5 : 3.0) + rounds * p.per * tile + (s > 1 ? 2.5 + (s + 1.0) * n * k * 4 / 4.5e6 : 0.0);
+            const double tile = big ? 1.02 : form == 2 ? 0.27 : at_once < 2 ? 0.43 : (at_once < 3 ? 0.27 : 0.32) * at_once;
+            const double c = (big ? 6.5 : form == 2 ? 4.5 : 3.0) + rounds * p.per * tile + (s > 1 ? 4.0 + (1.5 * s + 1.0) * n * k * 4 / 4.5e6 : 0.0);
             if (cost < 0 || c < cost) {
                 cost = c;
                 best = p;
@@ -333,8 +368,9 @@ SWAT_API int swat_mx_linear_wgrad(const void* dY_bf16, int64_t dy_stride, const 
     p.dY = (const unsigned short*)dY_bf16; p.X = (const unsigned char*)x_codes; p.S = (const unsigned char*)x_scales; p.dW = pw; p.db = pb;
     p.rows = rows; p.ld = dy_stride; p.n = n_out; p.k = n_in; p.blocks = (n_in + 31) / 32;
     p.tiles_n = pl.tiles_n; p.tiles_k = pl.tiles_k; p.splits = pl.splits; p.tiles_per_split = pl.per;
-    if (pl.big) mx_wgrad_kernel<128, 256, 64, 64><<<(unsigned)grid, 512, 0, s>>>(p);
-    else mx_wgrad_kernel<64, 64, 32, 32><<<(unsigned)grid, 256, 0, s>>>(p);
+    if (pl.form == 1) mx_wgrad_kernel<128, 256, 64, 64, 1><<<(unsigned)grid, 512, 0, s>>>(p);
+    else if (pl.form == 2) mx_wgrad_kernel<64, 64, 32, 32, 2><<<(unsigned)grid, 512, 0, s>>>(p);
+    else mx_wgrad_kernel<64, 64, 32, 32, 1><<<(unsigned)grid, 256, 0, s>>>(p);
     if (pl.splits > 1) {
         const int64_t quads = (nk > n_out ? nk : n_out) / 4 + 1;
         mx_wgrad_join_kernel<<<(unsigned)((quads + 255) / 256), 256, 0, s>>>(pw, pb, dW, dbias, nk, n_out, pl.splits, nk % 4 == 0);

@@ -163,6 +163,12 @@ def test_weight_gradient(rows, n, k):
         assert mx.linear_wgrad(dy, m, out=out) is out and torch.equal(out, dw)
 
 
+@pytest.mark.parametrize("rows,n,k", [(640, 65, 64), (833, 129, 100), (961, 64, 33), (1025, 255, 257), (1600, 769, 500), (2000, 63, 1000), (3201, 1000, 130)])
+def test_weight_gradient_of_few_tiles(rows, n, k):
+    """Two groups of waves share the rows: odd widths, an odd number of row tiles, a last tile of one row."""
+    test_weight_gradient(rows, n, k)
+
+
 def test_weight_gradient_leaves_what_is_not_its_own():
     """Rows of dY and columns behind a view are not read into the sums, outputs behind dW are left as they were."""
     from swat_amd import mx

@@ -3,7 +3,7 @@
 Tolerances.  A row's sums run over at most 16 values in a lane, 6 lane exchanges and 8 waves: 30 additions, each off by half a
 step (2^-24) of the running sum, which the sum of magnitudes bounds; the mean, the deviation, the root, the division and the few
 products behind them add under 30 more.  Outputs: 64 x 2^-24 of the magnitudes that enter plus half a step of the output's type;
-gradients through two norms twice that.  Column sums: the rows of a team (up to 7 here), 8 teams, 64 partial sums and 3: at most 82
+gradients through two norms twice that.  Column sums: the rows of a team (up to 7 here), 8 teams, 16 workgroups to a thread and 16 of those: at most 47
 additions over terms off by 64 x 2^-24 themselves: 256 x 2^-24 of the sum of magnitudes."""
 import pytest
 import torch
