@@ -38,26 +38,55 @@ __device__ __forceinline__ f32x4_t mx_mfma(mx_v8i b, mx_v8i a, f32x4_t c, int sb
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, a, c, BB == 4 ? 4 : 0, AB == 4 ? 4 : 0, S, sb, S, sa);
 }
 
-// lane holds C[m][n .. n + 3]
-__device__ __forceinline__ void mx_store4(const MxGemmArgs& p, int64_t m, int64_t n, f32x4_t v) {
-    if (m >= p.M || n >= p.N) return;
-    const int64_t at = m * p.N + n;
-    if (p.N % 4 == 0) {
-        if (p.bias) {
-            const float4 b = *reinterpret_cast<const float4*>(p.bias + n);
-            v[0] += b.x; v[1] += b.y; v[2] += b.z; v[3] += b.w;
-        }
-        if (p.out_bf) *reinterpret_cast<uint2*>((unsigned short*)p.C + at) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
-        else *reinterpret_cast<float4*>((float*)p.C + at) = make_float4(v[0], v[1], v[2], v[3]);
-        return;
-    }
+// bias[n .. n + 3] (columns past the last: anything, they are not stored)
+__device__ __forceinline__ f32x4_t mx_bias4(const MxGemmArgs& p, int64_t n) {
+    f32x4_t b = {0.f, 0.f, 0.f, 0.f};
+    if (p.bias) {
+        if (p.N % 4 == 0) {
+            if (n < p.N) b = *reinterpret_cast<const f32x4_t*>(p.bias + n);
+        } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-        if (n + e < p.N) {
-            const float t = p.bias ? v[e] + p.bias[n + e] : v[e];
-            if (p.out_bf) ((unsigned short*)p.C)[at + e] = f2bf(t);
-            else ((float*)p.C)[at + e] = t;
+            for (int e = 0; e < 4; ++e)
+                if (n + e < p.N) b[e] = p.bias[n + e];
         }
+    }
+    return b;
+}
+// A wave's tile: the lane holds C[m + 16 i][n + 16 j .. + 3].  What the whole launch shares is decided outside the loops and the bias is
+// loaded before the first store (which no load would be moved across).
+template <int FM, int FN>
+__device__ __forceinline__ void mx_store_tile(const MxGemmArgs& p, int64_t m, int64_t n, f32x4_t (&acc)[FM][FN]) {
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+        const f32x4_t b = mx_bias4(p, n + 16 * j);
+#pragma unroll
+        for (int i = 0; i < FM; ++i) acc[i][j] += b;
+    }
+    auto rows = [&](auto store) {
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+            if (m + 16 * i >= p.M) return;
+            const int64_t at = (m + 16 * i) * p.N + n;
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+                if (n + 16 * j < p.N) store(at + 16 * j, n + 16 * j, acc[i][j]);
+        }
+    };
+    unsigned short* const cb = (unsigned short*)p.C;
+    float* const cf = (float*)p.C;
+    if (p.N % 4 == 0) {
+        if (p.out_bf) rows([&](int64_t at, int64_t, f32x4_t v) { *reinterpret_cast<uint2*>(cb + at) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])); });
+        else rows([&](int64_t at, int64_t, f32x4_t v) { *reinterpret_cast<f32x4_t*>(cf + at) = v; });
+    } else {
+        rows([&](int64_t at, int64_t c, f32x4_t v) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (c + e < p.N) {
+                    if (p.out_bf) cb[at + e] = f2bf(v[e]);
+                    else cf[at + e] = v[e];
+                }
+        });
+    }
 }
 
 // 16 scale bytes of a row from block `first` on.  Rows sit on any byte: where 16 bytes would reach past the matrix's end (last: the row's last
@@ -271,10 +300,7 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, 2) void mx_gemm_kernel(
         bar();
         if (++t >= nk) break;
     }
-#pragma unroll
-    for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int j = 0; j < FN; ++j) mx_store4(p, m0 + WM * wr + 16 * i + r16, n0 + WN * wc + 16 * j + 4 * g, acc[i][j]);
+    mx_store_tile(p, m0 + WM * wr + r16, n0 + WN * wc + 4 * g, acc);
 }
 
 // The same for 4 by 4 bits in tiles of 128 and more, whose codes come straight into LDS, three tiles ahead, in a ring of four buffers: the loads
@@ -417,10 +443,7 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, 2) void mx_ring_kernel(
         if ((t += 2) >= nk) break;
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (no load may reach LDS after the workgroup has left it)
-#pragma unroll
-    for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int j = 0; j < FN; ++j) mx_store4(p, m0 + WM * wr + 16 * i + r16, n0 + WN * wc + 16 * j + 4 * g, acc[i][j]);
+    mx_store_tile(p, m0 + WM * wr + r16, n0 + WN * wc + 4 * g, acc);
 }
 
 // Few rows: a workgroup computes 16 columns of 16 FM rows, its 8 waves take the 128-column tiles of k in turn, straight from memory into
@@ -506,7 +529,8 @@ __global__ __launch_bounds__(512, 2) void mx_rows_kernel(MxGemmArgs p) {
         f32x4_t s = part[0][wave][lane];
 #pragma unroll
         for (int w = 1; w < 8; ++w) s += part[w][wave][lane];
-        mx_store4(p, p.m_begin + 16 * wave + r16, n0 + 4 * g, s);
+        f32x4_t one[1][1] = {{s}};
+        mx_store_tile(p, p.m_begin + 16 * wave + r16, n0 + 4 * g, one);
     }
 }
 
