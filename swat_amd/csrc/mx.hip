@@ -7,8 +7,9 @@
 // Storage: codes [rows, n rounded up to 32] (8 bits) or half of that (4 bits, the even column in the low half), scales
 // [rows, blocks of 32]; the columns behind n hold zeros, so every row starts on 32 (16) bytes and products need no edge along them.
 //
-// All of them are bound by bytes (8224 x 4096 there and back 5.5 and 6.3 TB/s; 16448 x 1024 fp32 to 4 bits 12.5 us, back 14.7).  A thread takes 8 neighbouring columns (16 bytes of bfloat16, 8 or 4 of codes), four lanes make
-// a block and agree on its scale by two lane exchanges.
+// All of them are bound by bytes: 8224 x 4096 with its checkpoint 31 us (5.4 TB/s), back 39 (6.0); 16448 x 1024 fp32 to 4 bits 13.4 us (5.7), back
+// 14.6 (5.2; a large copy 4.95).  A thread takes 8 neighbouring columns (16 bytes of bfloat16, 8 or 4 of codes), four lanes make a block and
+// agree on its scale by two lane exchanges.
 #include "gemm_device.hpp"
 #include "mx_device.hpp"
 #include "../../include/swat_hip.h"
