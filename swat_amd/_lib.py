@@ -124,6 +124,10 @@ def ptr(t):
     return t.data_ptr()
 
 
+# Kernels launch on the current device's current stream: a tensor on another device is refused instead of read from there.
+_current = torch._C._cuda_getDevice
+
+
 def rows_ptr(t, what, dtypes, cols=None):
     """(device pointer, row stride) of a 2-D GPU tensor on the current device whose rows are contiguous and do not overlap."""
     if isinstance(t, torch.Tensor) and t.dim() == 2 and t.dtype in dtypes and t.is_cuda and t.get_device() == _current():
@@ -149,11 +153,6 @@ def vec_ptr(t, what, *shape):
         got = f"{tuple(t.shape)} {t.dtype} on {t.device}" if isinstance(t, torch.Tensor) else repr(t)
         raise SwatHipError(f"{what}: a contiguous float32 GPU tensor of shape {shape} on the current device is wanted (no CPU fallback), got {got}")
     return t.data_ptr()
-
-
-def _current():
-    """Kernels launch on the current device's current stream: a tensor on another device is refused instead of read from there."""
-    return torch._C._cuda_getDevice()
 
 
 def stream():

@@ -5,6 +5,7 @@ they are (linear_wgrad, act_bwd); 4 bits halve that again for weights of frozen 
 multiplies any two of them without unpacking.  Thin wrappers over the C ABI (include/swat_hip.h) on torch's current stream; no
 PyTorch fallback.
 """
+import functools
 from collections import namedtuple
 
 import torch
@@ -12,7 +13,7 @@ import torch
 from . import _lib
 from .ops import ACT
 
-_BF, _F32 = torch.bfloat16, torch.float32
+_BF, _F32, _U8 = torch.bfloat16, torch.float32, torch.uint8
 _COLS = 1 << 24  # columns of a matrix at most (the C entries take them as 32-bit numbers)
 
 
@@ -32,17 +33,17 @@ class MX(namedtuple("MX", "codes scale cols bits")):
 
 def _empty(like, rows, cols, bits):
     blocks = (cols + 31) // 32
-    return MX(like.new_empty((rows, blocks * 4 * bits), dtype=torch.uint8), like.new_empty((rows, blocks), dtype=torch.uint8), cols, bits)
+    return MX(like.new_empty((rows, blocks * 4 * bits), dtype=_U8), like.new_empty((rows, blocks), dtype=_U8), cols, bits)
 
 
 def _check(m, what, bits=(4, 8)):
     """The pointers of an MX matrix whose parts fit together, on the current device."""
     if not isinstance(m, MX) or m.bits not in bits or not 1 <= m.cols <= _COLS:
         raise _lib.SwatHipError(f"{what}: an MX matrix of {' or '.join(map(str, bits))} bits and 1 to {_COLS} columns is wanted, got {m!r:.80}")
-    codes, scale = m.codes, m.scale
-    rows, blocks = codes.shape[0], (m.cols + 31) // 32
-    if (codes.dtype != torch.uint8 or scale.dtype != torch.uint8 or codes.shape != (rows, blocks * 4 * m.bits) or scale.shape != (rows, blocks)
-            or not codes.is_cuda or not scale.is_cuda or codes.get_device() != _lib._current() or scale.get_device() != _lib._current()
+    codes, scale, cols, nbits = m
+    rows, blocks, device = codes.shape[0], (cols + 31) // 32, codes.get_device()
+    if (device < 0 or device != scale.get_device() or device != _lib._current() or codes.dtype != _U8 or scale.dtype != _U8
+            or codes.shape != (rows, blocks * 4 * nbits) or scale.shape != (rows, blocks)
             or not codes.is_contiguous() or not scale.is_contiguous()):
         raise _lib.SwatHipError(f"{what}: codes {tuple(codes.shape)} {codes.dtype} on {codes.device}, scale {tuple(scale.shape)} {scale.dtype} on "
                                 f"{scale.device} are not the contiguous parts of {m.cols} columns in {m.bits} bits on the current device "
@@ -105,6 +106,11 @@ def act_bwd(dg, m, act="gelu", want_act=True):
     return df, g
 
 
+@functools.lru_cache(maxsize=256)
+def _wgrad_workspace(rows, n, cols):
+    return _lib.lib().swat_mx_linear_wgrad_workspace_bytes(rows, n, cols)
+
+
 def linear_wgrad(dy, m, want_bias=False, out=None):
     """Weight gradient from the 8-bit checkpoint of a linear layer's input: dy bf16 [rows, n] -> dW fp32 [n, cols] (, column sums of dy)."""
     codes, scale = _check(m, "mx.linear_wgrad", (8,))
@@ -116,10 +122,9 @@ def linear_wgrad(dy, m, want_bias=False, out=None):
         out = dy.new_empty((n, m.cols), dtype=_F32)
     pw = _lib.vec_ptr(out, "mx.linear_wgrad: out", n, m.cols)
     db = dy.new_empty(n, dtype=_F32) if want_bias else None
-    h = _lib.lib()
-    nbytes = h.swat_mx_linear_wgrad_workspace_bytes(rows, n, m.cols)
-    ws = dy.new_empty(nbytes, dtype=torch.uint8) if nbytes > 0 else None
-    _lib.check(h.swat_mx_linear_wgrad(py, ld, codes, scale, pw, db.data_ptr() if want_bias else None, rows, n, m.cols,
+    nbytes = _wgrad_workspace(rows, n, m.cols)
+    ws = dy.new_empty(nbytes, dtype=_U8) if nbytes > 0 else None
+    _lib.check(_lib.lib().swat_mx_linear_wgrad(py, ld, codes, scale, pw, db.data_ptr() if want_bias else None, rows, n, m.cols,
                                       ws.data_ptr() if nbytes > 0 else None, nbytes, _lib.stream()), "swat_mx_linear_wgrad")
     return (out, db) if want_bias else out
 

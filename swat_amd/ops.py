@@ -3,6 +3,7 @@
 Every function launches hand-written gfx950 kernels on torch's current stream and allocates only
 outputs; there is no PyTorch fallback.  bf16 tensors are torch.bfloat16, everything else fp32/int64.
 """
+import functools
 from collections import namedtuple
 
 import torch
@@ -155,6 +156,11 @@ def residual_norm_fwd(x, h, post=None, pre=None, gate=None, scale=None, alpha=1.
     return ResidualNorm(y, z, stats, z8)
 
 
+@functools.lru_cache(maxsize=256)
+def _seam_workspace(rows, d, groups, channels):
+    return _lib.lib().swat_residual_norm_bwd_workspace_bytes(rows, d, groups, channels)
+
+
 def residual_norm_bwd(dy, dz, h, y, stats, post=None, pre=None, gate=None, scale=None, alpha=1.0, norm="layer"):
     """Backward of residual_norm_fwd: dy (stream, may be None) and dz (None without pre) -> dict of gradients: 'x', 'h', and of what was
     given 'post_w', 'post_b', 'gate', 'scale', 'pre_w', 'pre_b'.  y, stats: the forward's (y may be None without pre).  Sums in a fixed order."""
@@ -184,10 +190,9 @@ def residual_norm_bwd(dy, dz, h, y, stats, post=None, pre=None, gate=None, scale
     if g is not None:
         out["gate"] = torch.empty_like(gate)
         dgate = out["gate"].data_ptr()
-    h_ = _lib.lib()
-    nbytes = h_.swat_residual_norm_bwd_workspace_bytes(rows, d, groups, channels)
+    nbytes = _seam_workspace(rows, d, groups, channels)
     ws = h.new_empty(nbytes, dtype=torch.uint8)
-    rc = h_.swat_residual_norm_bwd(pdy, sdy, pdz, sdz, dz is not None and dz.dtype == _BF, ph, sh, h.dtype == _BF, py, sy, xt == _BF, pst,
+    rc = _lib.lib().swat_residual_norm_bwd(pdy, sdy, pdz, sdz, dz is not None and dz.dtype == _BF, ph, sh, h.dtype == _BF, py, sy, xt == _BF, pst,
                                    *v[:8], float(alpha), rms, out["x"].data_ptr(), out["h"].data_ptr(), cols.get("post_w"), cols.get("post_b"),
                                    dgate, cols.get("scale"), cols.get("pre_w"), cols.get("pre_b"), ws.data_ptr(), nbytes, rows, d, _lib.stream())
     _chk(rc, "swat_residual_norm_bwd")
