@@ -269,31 +269,30 @@ __global__ __launch_bounds__((BN / WN) * (BK / WK) * 64 * GROUPS, 2) void mx_wgr
     }
 }
 
-// the planes of a split reduction, added in their order: dW behind which db follows in planes of its own
-__global__ __launch_bounds__(256) void mx_wgrad_join_kernel(const float* pw, const float* pb, float* dW, float* db, int64_t nk, int n, int splits, int vec) {
-    const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-    if (at < nk) {
-        if (vec) {
-            float4 s = *reinterpret_cast<const float4*>(pw + at);
-            for (int i = 1; i < splits; ++i) {
-                const float4 t = *reinterpret_cast<const float4*>(pw + i * nk + at);
-                s.x += t.x; s.y += t.y; s.z += t.z; s.w += t.w;
-            }
-            *reinterpret_cast<float4*>(dW + at) = s;
-        } else {
-            for (int e = 0; e < 4 && at + e < nk; ++e) {
-                float s = pw[at + e];
-                for (int i = 1; i < splits; ++i) s += pw[i * nk + at + e];
-                dW[at + e] = s;
-            }
+// the planes of a split reduction, added in their order, eight loads under way at a time: dW's in the first w_blocks workgroups, db's (behind
+// dW's in the workspace) in the others.  Four neighbours to a thread at any alignment; the last four of a count that is no multiple of 4
+// are made twice, to the same values.  (Element by element with a load at a time: 6980 x 32 x 35 16.5 us in all instead of 10.)
+typedef float mx_f4 __attribute__((ext_vector_type(4), aligned(4)));
+__global__ __launch_bounds__(256) void mx_wgrad_join_kernel(const float* pw, const float* pb, float* dW, float* db, int64_t nk, int n, int splits, int w_blocks) {
+    const bool w = (int)blockIdx.x < w_blocks;
+    const float* from = w ? pw : pb;
+    float* const to = w ? dW : db;
+    const int64_t count = w ? nk : n;
+    int64_t at = ((int64_t)(w ? (int)blockIdx.x : (int)blockIdx.x - w_blocks) * 256 + threadIdx.x) * 4;
+    if (at >= count) return;
+    if (count < 4) {
+        for (int e = 0; e < count; ++e) {
+            float s = from[e];
+            for (int i = 1; i < splits; ++i) s += from[i * count + e];
+            to[e] = s;
         }
+        return;
     }
-    if (db && at < n)
-        for (int e = 0; e < 4 && at + e < n; ++e) {
-            float s = pb[at + e];
-            for (int i = 1; i < splits; ++i) s += pb[(int64_t)i * n + at + e];
-            db[at + e] = s;
-        }
+    if (at + 4 > count) at = count - 4;
+    mx_f4 s = *reinterpret_cast<const mx_f4*>(from + at);
+#pragma unroll 8
+    for (int i = 1; i < splits; ++i) s += *reinterpret_cast<const mx_f4*>(from + i * count + at);
+    *reinterpret_cast<mx_f4*>(to + at) = s;
 }
 
 struct MxWgradPlan {
@@ -302,9 +301,9 @@ struct MxWgradPlan {
 };
 // 128 x 256 tiles (8 waves, one workgroup to a CU), 64 x 64 (4 waves, up to four) or, while those are one to a CU, 64 x 64 in two groups of
 // waves, and into how many parts the rows are split, by the sum of what was measured (us): a 64-row tile takes 1.02 in the first form, 0.43
-// in the second alone on its CU and 0.27 for each of several; 6.5 / 3 to start and to store; a join of parts 4 and its planes' bytes at 4.5
+// in the second alone on its CU and 0.27 for each of several; 6.5 / 3 to start and to store; a join of up to 32 parts 3.2 and its planes' bytes at 4.5
 // TB/s.  At 16448 rows, 4096 x 1024: 150 in the first form with 2 parts (259 with 1, 157 with 4), 240 in the second; at 1600 rows,
-// 768 x 768: 12.5 in two groups, 15 in one (2, 3, 4 parts: 15.3, 14.5, 16.9), 21.4 in the first; 6304 rows: 47.8 in one part, 35, 27.4, 28.4 in more.
+// 768 x 768: 12.5 in two groups, 15 in one (3 parts 14.5), 21.4 in the first; 6304 rows: 47.8 in one part, 26.8 in 3.
 static MxWgradPlan mx_wgrad_plan(int64_t rows, int n, int k) {
     const int64_t all = (rows + 63) / 64;
     MxWgradPlan best = {};
@@ -313,7 +312,7 @@ static MxWgradPlan mx_wgrad_plan(int64_t rows, int n, int k) {
         const bool big = form == 1;
         const int bn = big ? 128 : 64, bk = big ? 256 : 64;
         MxWgradPlan p = {form, (n + bn - 1) / bn, (k + bk - 1) / bk, 1, 1};
-        for (int s = 1; s <= 16 && (s == 1 || s <= all); ++s) {
+        for (int s = 1; s <= 32 && (s == 1 || s <= all); ++s) {
             p.per = all > 0 ? (int)((all + s - 1) / s) : 1;
             p.splits = all > 0 ? (int)((all + p.per - 1) / p.per) : 1;
             if (p.splits != s) continue;
@@ -321,7 +320,7 @@ static MxWgradPlan mx_wgrad_plan(int64_t rows, int n, int k) {
             if (form == 2 && units > 256) continue;
             const double at_once = units > 1024 ? 4 : ceil(units / 256);
             const double tile = big ? 1.02 : form == 2 ? 0.27 : at_once < 2 ? 0.43 : (at_once < 3 ? 0.27 : 0.32) * at_once;
-            const double c = (big ? 6.5 : form == 2 ? 4.5 : 3.0) + rounds * p.per * tile + (s > 1 ? 4.0 + (1.5 * s + 1.0) * n * k * 4 / 4.5e6 : 0.0);
+            const double c = (big ? 6.5 : form == 2 ? 4.5 : 3.0) + rounds * p.per * tile + (s > 1 ? 3.2 + (1.5 * s + 1.0) * n * k * 4 / 4.5e6 : 0.0);
             if (cost < 0 || c < cost) {
                 cost = c;
                 best = p;
@@ -372,8 +371,8 @@ SWAT_API int swat_mx_linear_wgrad(const void* dY_bf16, int64_t dy_stride, const 
     else if (pl.form == 2) mx_wgrad_kernel<64, 64, 32, 32, 2><<<(unsigned)grid, 512, 0, s>>>(p);
     else mx_wgrad_kernel<64, 64, 32, 32, 1><<<(unsigned)grid, 256, 0, s>>>(p);
     if (pl.splits > 1) {
-        const int64_t quads = (nk > n_out ? nk : n_out) / 4 + 1;
-        mx_wgrad_join_kernel<<<(unsigned)((quads + 255) / 256), 256, 0, s>>>(pw, pb, dW, dbias, nk, n_out, pl.splits, nk % 4 == 0);
+        const int64_t w_blocks = (nk + 1023) / 1024, b_blocks = dbias ? (n_out + 1023) / 1024 : 0;
+        mx_wgrad_join_kernel<<<(unsigned)(w_blocks + b_blocks), 256, 0, s>>>(pw, pb, dW, dbias, nk, n_out, pl.splits, (int)w_blocks);
     }
     return check_launch("swat_mx_linear_wgrad");
 }

@@ -169,6 +169,12 @@ def test_weight_gradient_of_few_tiles(rows, n, k):
     test_weight_gradient(rows, n, k)
 
 
+@pytest.mark.parametrize("rows,n,k", [(5000, 1, 1), (20000, 3, 1), (6980, 32, 35), (12745, 161, 61), (4052, 187, 701), (1738, 1917, 34), (9000, 5, 129)])
+def test_weight_gradient_of_many_parts(rows, n, k):
+    """Planes of any size and alignment are joined: fewer than four elements, a last four that overlaps the one before."""
+    test_weight_gradient(rows, n, k)
+
+
 def test_weight_gradient_leaves_what_is_not_its_own():
     """Rows of dY and columns behind a view are not read into the sums, outputs behind dW are left as they were."""
     from swat_amd import mx
