@@ -39,20 +39,20 @@ __device__ __forceinline__ f32x4_t mx_mfma(mx_v8i b, mx_v8i a, f32x4_t c, int sb
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, a, c, BB == 4 ? 4 : 0, AB == 4 ? 4 : 0, S, sb, S, sa);
 }
 
-// bias[n .. n + 3] (columns past the last: anything, they are not stored)
+// bias[n .. n + 3], n a multiple of 4 (columns past the last: zeros)
 __device__ __forceinline__ f32x4_t mx_bias4(const MxGemmArgs& p, int64_t n) {
     f32x4_t b = {0.f, 0.f, 0.f, 0.f};
     if (p.bias) {
-        if (p.N % 4 == 0) {
-            if (n < p.N) b = *reinterpret_cast<const f32x4_t*>(p.bias + n);
-        } else {
+        if (n + 4 <= p.N) b = *reinterpret_cast<const f32x4_t*>(p.bias + n);
+        else
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
+            for (int e = 0; e < 3; ++e)
                 if (n + e < p.N) b[e] = p.bias[n + e];
-        }
     }
     return b;
 }
+typedef unsigned mx_u2h __attribute__((ext_vector_type(2), aligned(2)));
+typedef float mx_f4f __attribute__((ext_vector_type(4), aligned(4)));
 // A wave's tile: the lane holds C[m + 16 i][n + 16 j .. + 3].  What the whole launch shares is decided outside the loops and the bias is
 // loaded before the first store (which no load would be moved across).
 template <int FM, int FN>
@@ -63,31 +63,27 @@ __device__ __forceinline__ void mx_store_tile(const MxGemmArgs& p, int64_t m, in
 #pragma unroll
         for (int i = 0; i < FM; ++i) acc[i][j] += b;
     }
-    auto rows = [&](auto store) {
+    auto rows = [&](auto four, auto one) {   // (rows start on any element where N is no multiple of 4)
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
             if (m + 16 * i >= p.M) return;
             const int64_t at = (m + 16 * i) * p.N + n;
 #pragma unroll
-            for (int j = 0; j < FN; ++j)
-                if (n + 16 * j < p.N) store(at + 16 * j, n + 16 * j, acc[i][j]);
+            for (int j = 0; j < FN; ++j) {
+                if (n + 16 * j + 4 <= p.N) four(at + 16 * j, acc[i][j]);
+                else
+#pragma unroll
+                    for (int e = 0; e < 3; ++e)
+                        if (n + 16 * j + e < p.N) one(at + 16 * j + e, acc[i][j][e]);
+            }
         }
     };
     unsigned short* const cb = (unsigned short*)p.C;
     float* const cf = (float*)p.C;
-    if (p.N % 4 == 0) {
-        if (p.out_bf) rows([&](int64_t at, int64_t, f32x4_t v) { *reinterpret_cast<uint2*>(cb + at) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])); });
-        else rows([&](int64_t at, int64_t, f32x4_t v) { *reinterpret_cast<f32x4_t*>(cf + at) = v; });
-    } else {
-        rows([&](int64_t at, int64_t c, f32x4_t v) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (c + e < p.N) {
-                    if (p.out_bf) cb[at + e] = f2bf(v[e]);
-                    else cf[at + e] = v[e];
-                }
-        });
-    }
+    if (p.out_bf)
+        rows([&](int64_t at, f32x4_t v) { *reinterpret_cast<mx_u2h*>(cb + at) = (mx_u2h){pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])}; },
+             [&](int64_t at, float v) { cb[at] = f2bf(v); });
+    else rows([&](int64_t at, f32x4_t v) { *reinterpret_cast<mx_f4f*>(cf + at) = v; }, [&](int64_t at, float v) { cf[at] = v; });
 }
 
 // 16 scale bytes of a row from block `first` on.  Rows sit on any byte: where 16 bytes would reach past the matrix's end (last: the row's last
