@@ -12,7 +12,7 @@
 //
 // Bound by bytes in both directions.  fp32 stream, bf16 branch, gate, scale and both norms (us, and TB/s of what has to move; a large copy
 // reaches 4.95): forward 16448 x 1024 46 (4.4), 12608 x 768 30 (3.8); backward 16448 x 1024 80 (3.8), 12608 x 768 48 (3.6), which adds
-// the column sums of up to five vectors.  50 x 768 takes 5 and 9 on the device: launches and latency.
+// the column sums of up to five vectors (5 of the 48).  50 x 768 forward: 6 on the device, one row's latency.
 #include <type_traits>
 #include "kernels.hpp"
 #include "mx_device.hpp"
