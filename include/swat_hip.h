@@ -541,7 +541,8 @@ int swat_mx_linear_wgrad(const void* dY_bf16, int64_t dy_stride, const void* x_c
 /* C [M, N] = A B^T (+ bias fp32 [N]) of packed A [M, K], B [N, K], 4 or 8 bits each, on the scaled matrix instructions (nothing is
  *     unpacked; fp32 accumulation).  c_dtype bf16, or fp32 where both operands have 4 bits: with an 8-bit operand the instruction drops
  *     what lies more than 13 binary places below the largest of eight neighbouring columns' products, far under the operands' own
- *     rounding (2^-4) and bf16's (2^-8), but not under fp32's.  Codes, bias and C sit on 16 bytes; K <= 2^22, M and N <= 2^30 and
+ *     rounding (2^-4) and bf16's (2^-8), but not under fp32's (sums in 32 bits: swat_mx_dequantize both to bf16, exactly, and
+ *     swat_gemm_bf16).  Codes, bias and C sit on 16 bytes; K <= 2^22, M and N <= 2^30 and
  *     fewer than 2^23 tiles (refused otherwise). */
 int swat_mx_matmul(const void* a_codes, const void* a_scales, int a_bits, const void* b_codes, const void* b_scales, int b_bits,
                    const float* bias, void* c, int c_dtype, int64_t M, int64_t N, int K, swat_stream_t stream);
