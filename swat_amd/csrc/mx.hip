@@ -7,9 +7,9 @@
 // Storage: codes [rows, n rounded up to 32] (8 bits) or half of that (4 bits, the even column in the low half), scales
 // [rows, blocks of 32]; the columns behind n hold zeros, so every row starts on 32 (16) bytes and products need no edge along them.
 //
-// All of them are bound by bytes: 8224 x 4096 with its checkpoint 31 us (5.4 TB/s), back 39 (6.0); 16448 x 1024 fp32 to 4 bits 13.4 us (5.7), back
-// 14.6 (5.2; a large copy 4.95).  A thread takes 8 neighbouring columns (16 bytes of bfloat16, 8 or 4 of codes), four lanes make a block and
-// agree on its scale by two lane exchanges.
+// All but GELU's forward (see mx_act) are bound by bytes: 8224 x 4096 QuickGELU with its checkpoint 27.5 us (6.1 TB/s), back 39 (6.0);
+// 16448 x 1024 fp32 to 4 bits 13.4 us (5.7), back 14.6 (5.2; a large copy 4.95).  A thread takes 8 neighbouring columns (16 bytes of
+// bfloat16, 8 or 4 of codes), four lanes make a block and agree on its scale by two lane exchanges.
 #include "gemm_device.hpp"
 #include "mx_device.hpp"
 #include "../../include/swat_hip.h"
@@ -147,10 +147,11 @@ __global__ __launch_bounds__(256) void mx_dequantize_kernel(MxMap m, const unsig
     mx_store8(out, bf, row * m.n + col, m.n - col, v);
 }
 
-// act(x) and act'(x).  GELU: the normal distribution's tail by Abramowitz & Stegun 7.1.26, erfc(z) = (a1 t + .. + a5 t^5) exp(-z^2),
-// t = 1 / (1 + p z), off by 1.5e-7 at most (a bfloat16 result shows 2e-3); its exponential is the density's that the slope needs as well,
-// so one exponential and one reciprocal serve both (8224 x 4096, with the library's erf: forward 37 us, backward 60, bound by arithmetic;
-// so 31 and 38, bound by bytes).
+// act(x) and act'(x).  GELU: the normal distribution's tail is exp(-z^2) erfcx(z) / 2, z = |x| / sqrt 2, and erfcx(z) / 2 = t (c1 + c2 t + .. + c7 t^6),
+// t = 1 / (1 + 0.512 z), with c fitted to the smallest largest RELATIVE error on 0 <= z <= 10 (a linear program): 7.7e-7, 1.1e-6 in fp32
+// arithmetic, so that the tail's bfloat16 result is good to its half step down to where exp(-z^2) ends (x = -13).  Its exponential is the
+// density's that the slope needs as well: one exponential and one reciprocal serve both.  8224 x 4096 there and back 73 us (105 with the
+// library's erfc); the forward alone, call after call, 40 where QuickGELU takes 27.5: bound by arithmetic.
 __device__ __forceinline__ void mx_act(float x, int act, float& value, float& slope) {
     if (act == 1) {
         const float s = __builtin_amdgcn_rcpf(1.0f + __expf(-1.702f * x));
@@ -159,9 +160,10 @@ __device__ __forceinline__ void mx_act(float x, int act, float& value, float& sl
         return;
     }
     const float z = fabsf(x) * 0.70710678118654752f, e = __expf(-0.5f * x * x);
-    const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, z, 1.0f));
-    const float poly = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
-    const float tail = 0.5f * poly * e, cdf = x < 0.f ? tail : 1.0f - tail;
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.512f, z, 1.0f));
+    const float poly = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.0478386469f, -0.179616824f), 0.175997242f), 0.0292394273f), 0.139293984f),
+                                             0.142730072f), 0.14451763f);
+    const float tail = poly * e, cdf = x < 0.f ? tail : 1.0f - tail;
     value = x * cdf;
     slope = fmaf(x * 0.39894228040143268f, e, cdf);
 }
