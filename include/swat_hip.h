@@ -520,7 +520,8 @@ int swat_residual_norm_bwd(const void* dy, int64_t dy_stride, const void* dz, in
  *     normal bfloat16); elements are x 2^-E rounded to nearest even.  A block that held a NaN or an infinity is NaN as a whole
  *     (byte 255).  codes uint8 [rows, ceil(n / 32) * 32 * bits / 8] (4 bits: the even column in the low half; the columns behind n
  *     are zeros), on 16 bytes; scales uint8 [rows, ceil(n / 32)].  1 <= n <= 2^24; values start on any element.  (In the top binade a
- *     number can round up to 2^128, which fp32 and bf16 hold as infinity.) */
+ *     number can round up to 2^128, which fp32 and bf16 hold as infinity.)  Packing writes scale bytes of 17 and more; the other entries
+ *     take every byte as it says, and round where values under 2^-126 become bf16. */
 int swat_mx_quantize(const void* x, int64_t x_stride, int x_dtype, int bits, void* codes, void* scales, int64_t rows, int n,
                      swat_stream_t stream);
 int swat_mx_dequantize(const void* codes, const void* scales, int bits, void* out, int out_dtype, int64_t rows, int n,

@@ -4,7 +4,8 @@
 // The scale of a block is the smallest power of two 2^E, E >= -110, with max |x| 2^-E <= the format's largest number: nothing
 // saturates, and the largest element keeps the format's full precision or all but one bit of it.  E >= -110 keeps every held value
 // a normal bfloat16 (the smallest e4m3 number is 2^-9), so unpacking is exact in bfloat16 and the matrix cores see what was stored.
-// Byte E + 127; byte 255: the block held a NaN or an infinity and is NaN as a whole.
+// Byte E + 127; byte 255: the block held a NaN or an infinity and is NaN as a whole.  A matrix put together by hand may have bytes under
+// 17: they mean what they say, but bfloat16 rounds such small values where they are unpacked to it.
 #pragma once
 #include "common.hpp"
 
@@ -31,7 +32,11 @@ __device__ __forceinline__ int mx_scale_byte(float top) {
     const int e = (int)(u >> 23) - 127 + (BITS == 8 ? -8 + ((u & 0x7fffffu) > 0x600000u) : -2 + ((u & 0x7fffffu) > 0x400000u));
     return (e < -110 ? -110 : e) + 127;
 }
-__device__ __forceinline__ float mx_scale(int byte) { return byte == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float((unsigned)byte << 23); }
+// (byte 0, which packing never writes: 2^-127, as the matrix instruction reads it, a subnormal float)
+__device__ __forceinline__ float mx_scale(int byte) {
+    const unsigned u = (unsigned)byte << 23;
+    return byte == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float(u > 0x400000u ? u : 0x400000u);
+}
 __device__ __forceinline__ float mx_inverse(int byte) { return __uint_as_float((unsigned)(254 - byte) << 23); }  // 2^-E (byte < 255)
 
 // four values to e4m3 / eight to e2m1, round to nearest even

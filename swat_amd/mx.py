@@ -19,7 +19,9 @@ _COLS = 1 << 24  # columns of a matrix at most (the C entries take them as 32-bi
 
 class MX(namedtuple("MX", "codes scale cols bits")):
     """A packed [rows, cols] matrix: codes uint8 [rows, ceil(cols / 32) * 32 * bits / 8] (4 bits: the even column in the low half, zeros
-    behind the last column), scale uint8 [rows, ceil(cols / 32)] (exponent + 127; 255: the block is NaN)."""
+    behind the last column), scale uint8 [rows, ceil(cols / 32)] (exponent + 127; 255: the block is NaN).  Packing takes the smallest power
+    of two that keeps a block within the format (other software may take the largest element's and cut off what is past the end) and
+    writes bytes of 17 or more; in a matrix put together by hand, values under smaller bytes are rounded where they become bf16."""
     __slots__ = ()
 
     @property
@@ -69,7 +71,7 @@ def quantize(x, bits=8):
 
 
 def dequantize(m, dtype=_BF):
-    """The values an MX matrix stands for, [rows, cols] in bf16 or fp32 (exact in both)."""
+    """The values an MX matrix stands for, [rows, cols] in bf16 or fp32 (exact in both; in bf16 from scale byte 17 on)."""
     codes, scale = _check(m, "mx.dequantize")
     if dtype not in (_BF, _F32):
         raise _lib.SwatHipError(f"mx.dequantize: {dtype} (bfloat16 or float32)")
