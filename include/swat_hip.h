@@ -489,7 +489,8 @@ int swat_preprocess_batch(const void* pixels_u8, const int64_t* offsets, const i
  *       p = Norm_post(h) (post_w null: h)      m = gate * scale (each may be null: 1)
  *       y = alpha x + m p                      z = Norm_pre(y)  (pre_w null: no z)
  *     Norm: LayerNorm, or root mean square (rms != 0); weights (and biases, may be null) fp32 [d], eps inside the root.  z is the
- *     norm of y as stored.  Where m is zero nothing of h is taken, whatever it holds (a dropped row may be NaN).
+ *     norm of y as stored.  Where m is zero nothing of p is taken: without Norm_post h may hold anything there, NaN too; with it only in
+ *     rows where all of m is zero (dropped rows), for in any other row each element has its share in the mean and the deviation.
  *     gate fp32: one number (gate_channels = 0: [groups]) or one row ([groups, d]) to rows / groups neighbouring rows; groups divides
  *     rows.  x and y share x_dtype; x, h: row strides in elements, d at least; y, z: contiguous.  stats fp32 [4][rows] (may be null):
  *     mean and 1 / deviation of Norm_post, of Norm_pre — what the backward call reads; rows of a norm that is not there stay as they
@@ -503,7 +504,8 @@ int swat_residual_norm_fwd(const void* x, int64_t x_stride, int x_dtype, const v
                            swat_stream_t stream);
 /*     its backward: dy (may be null: zero; x_dtype) and dz (z_dtype; null without pre_w) -> dx (x_dtype), dh (h_dtype) and the
  *     gradients of everything that was given (a pointer may be null to leave one out; dgate goes with gate).  y: the forward's
- *     output.  All sums in a fixed order (deterministic); gradients are written, not accumulated.  dh is zero where m is zero, and so is
+ *     output.  All sums in a fixed order (deterministic); gradients are written, not accumulated.  dh is zero where m is zero — with
+ *     Norm_post in rows where all of m is, elsewhere such an element's dh is its share through the mean and the deviation — and so is
  *     what such an element gives the norm's weights; a gate's gradient leaves out channels whose scale is zero, a scale's rows whose
  *     gate is zero (a zero gate's own gradient is what its branch holds).
  *     workspace: swat_residual_norm_bwd_workspace_bytes(rows, d, groups (0: no gate), gate_channels) bytes on 16 bytes. */

@@ -2,8 +2,9 @@
 //
 //   p = Norm_post(h)  (or h);   m = gate * scale;   y = alpha x + m p;   z = Norm_pre(y)
 //
-// Norm: LayerNorm or root mean square, eps inside the root.  An element whose multiplier m is zero takes nothing from the branch
-// (h is not looked at: a dropped row may hold anything).  z is the norm of the stream AS STORED, because the next sublayer's
+// Norm: LayerNorm or root mean square, eps inside the root.  An element whose multiplier m is zero takes nothing from p: h may
+// hold anything there without Norm_post, and in a row where all of m is zero (a dropped row) with it; in other rows Norm_post's mean and
+// deviation are over every element, which then has its share of dh through them.  z is the norm of the stream AS STORED, because the next sublayer's
 // backward pass reads that y.
 //
 // A row lives in the registers of one team of W waves; both norms take their mean and their squared deviations from there, so

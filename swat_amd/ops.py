@@ -133,7 +133,7 @@ def residual_norm_fwd(x, h, post=None, pre=None, gate=None, scale=None, alpha=1.
     x [rows, d] the residual stream and h [rows, d] what the sublayer returned, bf16 or fp32 each (rows may be strided); post, pre:
     (weight, bias or None) fp32 [d], or None for no such norm (no pre: z is None); norm 'layer' | 'rms'; scale fp32 [d]; gate fp32
     [groups] or [groups, d], for rows / groups neighbouring rows each (stochastic depth: 0 or 1 / keep per image).  Where gate * scale is
-    zero nothing of h is taken.  y has x's type, z z_dtype; stats fp32 [4, rows] is for residual_norm_bwd; pack: z8 = z as an 8-bit
+    zero nothing of the branch is taken: without post h may hold anything there (NaN), with post in rows where all of it is zero.  y has x's type, z z_dtype; stats fp32 [4, rows] is for residual_norm_bwd; pack: z8 = z as an 8-bit
     microscaled matrix (mx.MX), the checkpoint of the next linear layer's input or an operand of mx.matmul."""
     px, sx = _lib.rows_ptr(x, "residual_norm_fwd: x", (_BF, _F32))
     rows, d = x.shape
