@@ -124,8 +124,9 @@ def ptr(t):
     return t.data_ptr()
 
 
-# Kernels launch on the current device's current stream: a tensor on another device is refused instead of read from there.
-_current = torch._C._cuda_getDevice
+# Kernels launch on the current device's current stream: a tensor on another device is refused instead of read from there.  (The names
+# under torch._C are missing from a torch without GPU support, where no tensor gets as far as to need them.)
+_current = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def rows_ptr(t, what, dtypes, cols=None):
@@ -156,4 +157,5 @@ def vec_ptr(t, what, *shape):
 
 
 def stream():
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())  # (current_stream().cuda_stream without the Stream object: 0.4 us, not 2.9)
+    device = torch.cuda.current_device()
+    return torch._C._cuda_getCurrentRawStream(device)  # (current_stream().cuda_stream without the Stream object: 0.4 us, not 2.9)
