@@ -536,7 +536,7 @@ int swat_mx_act_bwd(const void* dg_bf16, int64_t dg_stride, const void* codes, c
                     int64_t rows, int n, swat_stream_t stream);
 /* Weight gradient of a linear layer whose input was kept as an 8-bit checkpoint: dW [n_out, n_in] = dY^T X8 (fp32, written),
  *     dbias [n_out] = column sums of dY (may be null).  dY bf16 [rows, n_out] with a row stride.  Unpacking is exact, accumulation
- *     fp32, the order of the sums fixed.  dY starts on any element, its row stride is 2^23 at most; n_in <= 2^24, n_out n_in < 2^34; dW sits
+ *     fp32, the order of the sums fixed.  dY starts on any element, its row stride is 2^23 at most; 1 <= n_in <= 2^24, n_out n_in < 2^34; dW sits
  *     on 16 bytes.  workspace: swat_mx_linear_wgrad_workspace_bytes(...) bytes on 16 bytes (0: null will do). */
 int64_t swat_mx_linear_wgrad_workspace_bytes(int64_t rows, int n_out, int n_in);
 int swat_mx_linear_wgrad(const void* dY_bf16, int64_t dy_stride, const void* x_codes, const void* x_scales, float* dW, float* dbias,

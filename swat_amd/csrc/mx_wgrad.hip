@@ -335,7 +335,7 @@ static MxWgradPlan mx_wgrad_plan(int64_t rows, int n, int k) {
 using namespace swat;
 
 SWAT_API int64_t swat_mx_linear_wgrad_workspace_bytes(int64_t rows, int n_out, int n_in) {
-    if (rows < 0 || rows >= (1ll << 36) || n_out < 0 || n_in < 0 || n_out > (1 << 23) || n_in > (1 << 24)) {
+    if (rows < 0 || rows >= (1ll << 36) || n_out < 0 || n_in < 1 || n_out > (1 << 23) || n_in > (1 << 24)) {
         set_error("swat_mx_linear_wgrad_workspace_bytes: %lld rows, %d x %d", (long long)rows, n_out, n_in);
         return -1;
     }
@@ -345,8 +345,8 @@ SWAT_API int64_t swat_mx_linear_wgrad_workspace_bytes(int64_t rows, int n_out, i
 
 SWAT_API int swat_mx_linear_wgrad(const void* dY_bf16, int64_t dy_stride, const void* x_codes, const void* x_scales, float* dW, float* dbias,
                                   int64_t rows, int n_out, int n_in, void* workspace, int64_t workspace_bytes, swat_stream_t stream) {
-    SWAT_REQUIRE(rows >= 0 && rows < (1ll << 36) && n_out >= 0 && n_in >= 0 && n_out <= (1 << 23) && n_in <= (1 << 24), "swat_mx_linear_wgrad: %lld rows, %d x %d", (long long)rows, n_out, n_in);
-    if (n_out == 0 || n_in == 0) return 0;
+    SWAT_REQUIRE(rows >= 0 && rows < (1ll << 36) && n_out >= 0 && n_in >= 1 && n_out <= (1 << 23) && n_in <= (1 << 24), "swat_mx_linear_wgrad: %lld rows, %d x %d", (long long)rows, n_out, n_in);
+    if (n_out == 0) return 0;
     SWAT_REQUIRE(dW && (rows == 0 || (dY_bf16 && x_codes && x_scales)), "swat_mx_linear_wgrad: dY, the checkpoint and dW are needed");
     SWAT_REQUIRE(rows == 0 || dy_stride >= n_out, "swat_mx_linear_wgrad: row stride %lld under %d columns", (long long)dy_stride, n_out);
     SWAT_REQUIRE(rows == 0 || dy_stride <= (1 << 23), "swat_mx_linear_wgrad: row stride %lld past 2^23", (long long)dy_stride);
