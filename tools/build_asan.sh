@@ -7,7 +7,7 @@ set -e
 cd "$(dirname "$0")/../swat_amd/csrc"
 OBJ=_obj_asan
 mkdir -p $OBJ ../lib
-FLAGS="--offload-arch=gfx950 -O1 -g -fPIC -std=c++17 -fvisibility=hidden -fsanitize=address,undefined -fno-gpu-sanitize -fno-omit-frame-pointer -fno-sanitize-recover=undefined"
+FLAGS="--offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O1 -g -fPIC -std=c++17 -fvisibility=hidden -fsanitize=address,undefined -fno-gpu-sanitize -fno-omit-frame-pointer -fno-sanitize-recover=undefined"
 n=0
 for f in *.hip; do
   o=$OBJ/${f%.hip}.o
