@@ -624,15 +624,15 @@ struct RnPlan {
 // columns, four up to 2 048, eight beyond, because it keeps more of a row and the column sums in registers (16448 x 1024 with a row of
 // gates: 75 us, 163 with one wave to a row and spilled registers); at most one workgroup of eight waves to each of the 256 CUs (two of
 // four, four where a lane has one vector): every workgroup leaves four rows of column sums, 2 to 8 % of what the rows are.
-static RnPlan rn_plan(int rows, int d, bool bwd) {
+static RnPlan rn_plan(int64_t rows, int d, bool bwd) {   // (64 bits: sums next to 2^31 rows)
     RnPlan p;
     p.W = d <= (bwd ? 768 : 1024) ? 1 : d <= (bwd ? 2048 : 4096) ? 4 : 8;
     const int need = (d + 256 * p.W - 1) / (256 * p.W);
     p.nch = need == 3 && p.W > 1 ? 4 : need;
     const int teams_blk = p.W == 1 ? 8 : 1, most = 256 * (p.W == 1 ? 8 : p.W == 4 ? (p.nch == 1 ? 4 : 2) : 1);
-    const int teams = rows < most ? rows : most;
-    p.rows_per_team = rows ? (rows + teams - 1) / teams : 1;
-    p.teams = rows ? (rows + p.rows_per_team - 1) / p.rows_per_team : 0;
+    const int64_t teams = rows < most ? rows : most;
+    p.rows_per_team = rows ? (int)((rows + teams - 1) / teams) : 1;
+    p.teams = rows ? (int)((rows + p.rows_per_team - 1) / p.rows_per_team) : 0;
     p.blocks = (p.teams + teams_blk - 1) / teams_blk;
     p.teams = p.blocks * teams_blk;
     return p;
