@@ -40,9 +40,11 @@ def _empty(like, rows, cols, bits):
 
 def _check(m, what, bits=(4, 8)):
     """The pointers of an MX matrix whose parts fit together, on the current device."""
-    if not isinstance(m, MX) or m.bits not in bits or not 1 <= m.cols <= _COLS:
+    if not isinstance(m, MX) or m.bits not in bits or not isinstance(m.cols, int) or not 1 <= m.cols <= _COLS:
         raise _lib.SwatHipError(f"{what}: an MX matrix of {' or '.join(map(str, bits))} bits and 1 to {_COLS} columns is wanted, got {m!r:.80}")
     codes, scale, cols, nbits = m
+    if not isinstance(codes, torch.Tensor) or not isinstance(scale, torch.Tensor) or codes.dim() != 2:
+        raise _lib.SwatHipError(f"{what}: codes {codes!r:.60} and scale {scale!r:.60} are not the parts of an MX matrix")
     rows, blocks, device = codes.shape[0], (cols + 31) // 32, codes.get_device()
     if (device < 0 or device != scale.get_device() or device != _lib._current() or codes.dtype != _U8 or scale.dtype != _U8
             or codes.shape != (rows, blocks * 4 * nbits) or scale.shape != (rows, blocks)
@@ -54,7 +56,7 @@ def _check(m, what, bits=(4, 8)):
 
 
 def _act(act, what):
-    if ACT.get(act, 0) == 0:
+    if not isinstance(act, str) or ACT.get(act, 0) == 0:
         raise _lib.SwatHipError(f"{what}: activation {act!r} ('gelu' or 'quick_gelu')")
     return ACT[act]
 

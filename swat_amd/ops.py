@@ -110,15 +110,16 @@ def _seam(what, rows, d, post, pre, gate, scale, norm):
         raise _lib.SwatHipError(f"{what}: norm {norm!r} ('layer' or 'rms')")
     if rows >= 1 << 31:
         raise _lib.SwatHipError(f"{what}: {rows} rows (under 2^31)")
+    for wb in (post, pre):
+        if wb is not None and (not isinstance(wb, (tuple, list)) or len(wb) != 2 or wb[0] is None):
+            raise _lib.SwatHipError(f"{what}: post, pre = (weight, bias or None)")
     pw, pb = post if post is not None else (None, None)
     qw, qb = pre if pre is not None else (None, None)
-    if (post is not None and pw is None) or (pre is not None and qw is None):
-        raise _lib.SwatHipError(f"{what}: post, pre = (weight, bias or None)")
     vec = _lib.vec_ptr
     g, groups, channels = None, 0, 0
     if gate is not None:
-        if gate.dim() not in (1, 2):
-            raise _lib.SwatHipError(f"{what}: gate is [groups] or [groups, d], got {tuple(gate.shape)}")
+        if not isinstance(gate, torch.Tensor) or gate.dim() not in (1, 2):
+            raise _lib.SwatHipError(f"{what}: gate is a tensor [groups] or [groups, d], got {tuple(gate.shape) if isinstance(gate, torch.Tensor) else gate!r:.80}")
         groups, channels = gate.shape[0], int(gate.dim() == 2)
         g = vec(gate, what, groups, d) if channels else vec(gate, what, groups)
         if groups < 1 or rows % groups:
@@ -168,10 +169,10 @@ def residual_norm_bwd(dy, dz, h, y, stats, post=None, pre=None, gate=None, scale
     rows, d = h.shape
     if (dz is None) != (pre is None) or (dy is None and dz is None) or (pre is not None and y is None) or not 1 <= d <= 8192:
         raise _lib.SwatHipError(f"residual_norm_bwd: dz and y go with pre, dy or dz is needed, 1 to 8192 columns (d = {d})")
-    xt = y.dtype if y is not None else dy.dtype
+    py, sy = _lib.rows_ptr(y, "residual_norm_bwd: y", (_BF, _F32), d) if y is not None else (None, d)
+    xt = y.dtype if y is not None else getattr(dy, "dtype", _F32)
     pdy, sdy = _lib.rows_ptr(dy, "residual_norm_bwd: dy", (xt,), d) if dy is not None else (None, d)
     pdz, sdz = _lib.rows_ptr(dz, "residual_norm_bwd: dz", (_BF, _F32), d) if dz is not None else (None, d)
-    py, sy = _lib.rows_ptr(y, "residual_norm_bwd: y", (_BF, _F32), d) if y is not None else (None, d)
     if (xt != _BF and xt != _F32) or any(t is not None and t.shape[0] != rows for t in (dy, dz, y)):
         raise _lib.SwatHipError("residual_norm_bwd: dy, dz, h and y have the same rows; the stream is bf16 or fp32")
     pst = _lib.vec_ptr(stats, "residual_norm_bwd: stats", 4, rows)
