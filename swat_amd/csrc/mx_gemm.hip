@@ -165,7 +165,8 @@ struct MxScales {
 // A workgroup computes BM x BN of C in waves of WM x WN, 128 columns at a time: codes go through registers into one of two LDS buffers while
 // the matrix cores work on the other, loads two tiles ahead.  A row's scales come 16 bytes (four tiles) at a time, are transposed to
 // [block of the tile][tile] and kept in LDS, so that one 4-byte read gives a lane the scales of its row and block for four tiles, which
-// the instruction picks by byte.  16384 x 1024 x 4096 in 256 x 256 (8 waves of 128 x 64): 8 by 8 bits 70 us, 8 by 4 61 (2.2 PFLOP/s).
+// the instruction picks by byte.  16384 x 1024 x 4096 in 256 x 256 (8 waves of 128 x 64): 8 by 8 bits 67 us (2.1
+// PFLOP/s; matrix pipes busy 45 % of the time by counter, LDS 31), 8 by 4 59.
 template <int AB, int BB, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, 2) void mx_gemm_kernel(MxGemmArgs p) {
     constexpr int NT = (BM / WM) * (BN / WN) * 64, FM = WM / 16, FN = WN / 16;
@@ -303,8 +304,8 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, 2) void mx_gemm_kernel(
 // The same for 4 by 4 bits in tiles of 128 and more, whose codes come straight into LDS, three tiles ahead, in a ring of four buffers: the loads
 // cost no registers, so that there is room to read the next tile's B and half of its A while this tile's second half multiplies, and they
 // may take the time of two tiles.  16448 x 1024 x 4096: 54.5 -> 47.7 us, 8192^3 323 -> 273 (4.0 PFLOP/s; in 128 x 128 405 -> 386).  Bound by
-// the matrix cores and LDS in turn: without loads and LDS reads 16384 x 1024 x 4096 takes 33 of its 46 us, of which 16 are what the
-// matrix instructions take from registers with every CU on them (8.7 PFLOP/s).
+// the matrix cores and LDS in turn (busy 42 and 37 % of the time by counter): 16384 x 1024 x 4096 takes 42 us, 72 % of its time without loads and
+// LDS reads, and 16 is what the matrix instructions take from registers with every CU on them (8.7 PFLOP/s).
 // What a load past an edge leaves in LDS (the next row's codes, zeros or older codes) is multiplied by block scales of zero bytes, 2^-127 on
 // both sides, or belongs to rows that are not stored: an e2m1 code is always finite.
 template <int BM, int BN, int WM, int WN>

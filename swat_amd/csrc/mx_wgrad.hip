@@ -6,8 +6,9 @@
 // checkpoint is unpacked on its way into LDS without a rounding and v_mfma_f32_16x16x32_bf16 sees what was stored.  The reduction
 // runs over rows: both tiles lie [64 rows][columns] in LDS and are read with the transposing LDS load.
 //
-// Bound by the matrix cores where it is large: 16448 rows, 4096 x 1024 takes 150 us (920 TFLOP/s; the large bf16 library product 1 425, the
-// same gradient from a bf16 input 149-179 with the GEMM kernels of gemm_*.hip), matrix pipes busy 44 % of the time by counter.  A wave's
+// 16448 rows, 4096 x 1024: 147 us call after call (940 TFLOP/s; kernel 139, join 8; the first twenty calls after a pause take 187 each, while the
+// clocks rise), the same gradient from a bf16 input, without db, 153 with the GEMM kernels of gemm_*.hip, the large bf16 library product 1 425 TFLOP/s.  By
+// counter a CU's matrix pipes work 43 % of the time, its LDS 37, its vector units 30: no unit is the bound, the turns they take are.  A wave's
 // 64 x 64 and 8 waves to a CU leave one other wave to a SIMD to cover LDS reads, LDS writes and the unpacking; wider wave tiles spilled.
 // The long side of the tile goes to X because its codes are half as many bytes: 32 KB instead of 40 from memory for the same products.
 #include <math.h>

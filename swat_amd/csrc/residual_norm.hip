@@ -12,8 +12,10 @@
 // columns of a width that is no multiple of 4 come as the row's last four, shifted down in registers.
 //
 // Bound by bytes in both directions.  fp32 stream, bf16 branch, gate, scale and both norms (us, and TB/s of what has to move; a large copy
-// reaches 4.95): forward 16448 x 1024 46 (4.4), 12608 x 768 30 (3.8); backward 16448 x 1024 80 (3.8), 12608 x 768 48 (3.6), which adds
-// the column sums of up to five vectors (5 of the 48).  50 x 768 forward: 6 on the device, one row's latency.
+// reaches 4.95): forward 16448 x 1024 44.5 (4.5; 49 with the packed z), 12608 x 768 28 (4.1), 4112 x 4096 45 (4.5), 2056 x 8192 50 (4.1); backward
+// 74 (4.1), 47.5 (3.7), 85 (3.5) and 114 (2.7: eight waves to a row, two barriers to a sum, one workgroup to a CU), which adds the column
+// sums of up to five vectors (5 of the 47.5).  All in fp32, backward: 92, 53, 108 and 165.  50 x 768 forward: 6 on the device, the latency
+// of loads that wait for each other.
 #include <type_traits>
 #include "kernels.hpp"
 #include "mx_device.hpp"
@@ -553,7 +555,8 @@ struct RnFinish {
 // workgroups 0 .. 3 col_blocks - 1: 16 columns of the sums that belong together (those of the norm before, d weight and d bias of the one
 // after), 16 threads to a column over a sixteenth of the blocks each, eight loads of a thread under way at a time (four threads to a
 // column took 19 us, as long as a quarter of the rows' pass); behind them the gate: 4 groups to a workgroup (a number per group) or 256
-// columns of one group (a row per group)
+// columns of one group (a row per group).  A group's rows are added by one wave, its parts of a row by one thread to a column: right for many
+// groups of few rows.  A gate shared by all of 16448 x 1024 takes the whole backward from 74 us to 127 (a number) or 108 (a row).
 __global__ __launch_bounds__(256) void residual_norm_finish_kernel(RnFinish f) {
     __shared__ float sh[2][16][17];
     int64_t b = blockIdx.x;
